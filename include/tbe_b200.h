@@ -46,7 +46,9 @@ typedef enum {
   TBE_ERR_TIMEOUT = -6           /* a bounded device-side wait ran out */
 } tbe_status_t;
 
-typedef enum { TBE_F32 = 0, TBE_F16 = 1, TBE_F64 = 2 } tbe_dtype_t;
+/* TBE_BF16 is taken by the expert-routing and gradient-clipping entry points only; tables are fp16, fp32
+ * or fp64. */
+typedef enum { TBE_F32 = 0, TBE_F16 = 1, TBE_F64 = 2, TBE_BF16 = 3 } tbe_dtype_t;
 typedef enum { TBE_POOL_SUM = 0, TBE_POOL_MEAN = 1 } tbe_pooling_t;
 
 #define TBE_MAX_PEERS 16
@@ -296,6 +298,67 @@ TBE_API int tbe_sort_segments(const int32_t* table_offsets, const int32_t* indic
                       int32_t* sorted_rows, int32_t* sorted_bags,
                       int32_t* segment_starts, int32_t* num_segments,
                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- expert routing: samples sorted by expert and back -------------------- */
+
+/* For models whose samples pass through a few of E experts.  The reference has no such layer.  dtype is
+ * any tbe_dtype_t; "weights" and their gradients are fp32 (fp64 for TBE_F64).  All arrays are device
+ * memory.  Rows may have any width; they move in the widest vectors (16 bytes down to one element) that
+ * the addresses and strides allow.  Limits: E <= 1024, k <= min(E, 32) in the gate, N*k < 2^31.
+ *
+ * tbe_expert_gate: logits [N][E] (rows row_stride elements apart) -> the k largest of every row,
+ * descending, ties to the lowest index: experts int32 [N][k], and weights [N][k]:
+ *   renormalize != 0: softmax over the chosen;  0: the softmax over the whole row at the chosen.
+ * A logit of -inf is never chosen: its slot gets id -1 and weight 0 (a row of nothing else: all -1, all
+ * 0).  NaN ranks above +inf; a row with a chosen NaN or +inf (renormalize = 0: with any) has NaN weights.
+ * tbe_expert_gate_backward: grad_logits [N][E] (contiguous) from grad_weights [N][k], the gate's
+ * results and (read only when renormalize = 0) its logits. */
+TBE_API int tbe_expert_gate(const void* logits, int64_t row_stride, void* weights, int32_t* experts, int64_t N,
+                            int64_t E, int64_t k, int dtype, int renormalize, void* stream);
+TBE_API int tbe_expert_gate_backward(const void* grad_weights, const void* logits, int64_t row_stride,
+                                     const void* weights, const int32_t* experts, void* grad_logits, int64_t N,
+                                     int64_t E, int64_t k, int dtype, int renormalize, void* stream);
+/* Stable sort of M choices (experts[M] = [N][k] flattened) by expert: positions[i] is the row choice i
+ * takes, order[positions[i]] = i, and rows offsets[e] .. offsets[e+1) (int32 [E+1]) are expert e's.  Ids
+ * outside 0..E-1 -- unassigned slots, experts of another rank -- sort behind all experts, at rows
+ * offsets[E] .. M-1.  One kernel for up to 8192 choices, two above (workspace:
+ * tbe_expert_plan_workspace_bytes, 0 for one kernel; it needs no initialisation). */
+TBE_API int64_t tbe_expert_plan_workspace_bytes(int64_t M, int64_t E);
+TBE_API int tbe_expert_plan(const int32_t* experts, int32_t* offsets, int32_t* positions, int32_t* order, int64_t M,
+                            int64_t E, void* workspace, int64_t workspace_bytes, void* stream);
+/* y[positions[t][s]][:] = x[t][:], rows from offsets[E] on are zero.  x [N][D] with rows row_stride
+ * elements apart, y [N*k][D] contiguous. */
+TBE_API int tbe_expert_dispatch(const void* x, int64_t row_stride, const int32_t* positions, const int32_t* offsets,
+                                void* y, int64_t N, int64_t k, int64_t D, int64_t E, int dtype, void* stream);
+/* out[t][:] = sum over the slots with positions[t][s] < offsets[E] of weights[t][s] * y[positions[t][s]][:],
+ * slots ascending, fp32 accumulation (fp64 for TBE_F64); weights NULL = 1, which is the gradient of
+ * tbe_expert_dispatch.  Rows of y from offsets[E] on are not read.  y [N*k][D] and out [N][D] contiguous. */
+TBE_API int tbe_expert_combine(const void* y, const int32_t* positions, const int32_t* offsets, const void* weights,
+                               void* out, int64_t N, int64_t k, int64_t D, int64_t E, int dtype, void* stream);
+/* grad_y[positions[t][s]][:] = weights[t][s] * grad_out[t][:] (zero from offsets[E] on) and
+ * grad_weights[t][s] = <grad_out[t], y[positions[t][s]]> (0 for slots that are not kept).  Either output
+ * may be NULL; y is only read for grad_weights. */
+TBE_API int tbe_expert_combine_backward(const void* grad_out, int64_t grad_stride, const void* y,
+                                        const int32_t* positions, const int32_t* offsets, const void* weights,
+                                        void* grad_y, void* grad_weights, int64_t N, int64_t k, int64_t D, int64_t E,
+                                        int dtype, void* stream);
+
+/* ---- gradients: global norm and clipping ----------------------------------- */
+
+/* norm (device, one float) = sqrt(sum of squares over all elements of `count` tensors), summed in fp64 in
+ * a fixed order.  tensors, numels and dtypes are HOST arrays, read during the call; every tensor is dense
+ * memory of numels[i] elements (0 is allowed) on the current device.  The table travels in the kernels'
+ * parameters, 1024 tensors per launch. */
+TBE_API int64_t tbe_grad_norm_workspace_bytes(int64_t count);
+TBE_API int tbe_grad_norm(const void* const* tensors, const int64_t* numels, const int32_t* dtypes, int64_t count,
+                          float* norm, void* workspace, int64_t workspace_bytes, void* stream);
+/* outputs[i] = min(1, max_norm / (norm + eps)) * tensors[i], rounded once; outputs[i] == tensors[i] is in
+ * place.  A norm of NaN makes everything NaN, an infinite one zeroes the finite elements, as the formula
+ * says.  With every tensor in place and a factor of 1 nothing is stored.  An output that shares memory
+ * with another tensor of the list is refused. */
+TBE_API int tbe_grad_clip(const void* const* tensors, void* const* outputs, const int64_t* numels, const int32_t* dtypes,
+                          int64_t count, double max_norm, double eps, float* norm, void* workspace,
+                          int64_t workspace_bytes, void* stream);
 
 /* ---- input helpers ------------------------------------------------------ */
 

@@ -9,12 +9,13 @@ import threading
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libtbe_b200.so")
 
-TBE_F32, TBE_F16, TBE_F64 = 0, 1, 2
+TBE_F32, TBE_F16, TBE_F64, TBE_BF16 = 0, 1, 2, 3
 TBE_POOL_SUM, TBE_POOL_MEAN = 0, 1
 TBE_MAX_PEERS = 16
 
 c_i32p = ctypes.POINTER(ctypes.c_int32)
 _vp, _i64, _i32, _f32, _u64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_uint64
+_f64 = ctypes.c_double
 
 # name -> (restype, argtypes); every symbol declared in include/tbe_b200.h
 SIGNATURES = {
@@ -49,6 +50,17 @@ SIGNATURES = {
                                                    _i64, _i64, _i64, _i32, _f32, _f32, _i32, _u64, _u64, _i64,
                                                    _vp, _i64, _vp]),
     "tbe_sort_segments": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "tbe_expert_gate": (_i32, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp]),
+    "tbe_expert_gate_backward": (_i32, [_vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp]),
+    "tbe_expert_plan_workspace_bytes": (_i64, [_i64, _i64]),
+    "tbe_expert_plan": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp]),
+    "tbe_expert_dispatch": (_i32, [_vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp]),
+    "tbe_expert_combine": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp]),
+    "tbe_expert_combine_backward": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32,
+                                           _vp]),
+    "tbe_grad_norm_workspace_bytes": (_i64, [_i64]),
+    "tbe_grad_norm": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp]),
+    "tbe_grad_clip": (_i32, [_vp, _vp, _vp, _vp, _i64, _f64, _f64, _vp, _vp, _i64, _vp]),
     "tbe_construct_offsets": (_i32, [_vp, _vp, _vp, _i64, _i64, _vp]),
     "tbe_permute_bags": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "tbe_check_inputs": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _vp]),

@@ -1,0 +1,356 @@
+// The router's gate: the k largest logits of every row with their softmax weights, and its gradient.
+//
+// Forward, per row l[0..E):   chosen = the k largest, ties to the lowest index, descending
+//   e_j = exp(l_j - max l);   w_s = e_s / sum over the chosen   (renormalize)
+//                             w_s = e_s / sum over all           (otherwise)
+// A logit of -inf is a switched-off expert: it is never chosen, its slot gets id -1 and weight 0, so a
+// row with nothing left is (-1, 0) throughout.  NaN ranks above everything and makes the row's weights
+// NaN, as the formula does; the ids stay distinct and in range.
+//
+// A row belongs to a group of G = 2^g lanes (several rows per warp when E is small), each lane holds V
+// of its logits as sort keys that carry the value's order and the column: the larger key is the larger
+// logit, or the lower column of equal ones.  16-bit logits fit value and column into 32 bits, so a warp
+// finds a maximum in one redux; 32-bit ones take 64-bit keys and two.  Each of the k rounds takes the
+// group's maximum and clears it where it is held.  Nothing but the logits is read and nothing is kept
+// for the backward, which recomputes the row's maximum and sum from the logits when it needs them.
+#include "tbe_elem.cuh"
+
+namespace tbe {
+namespace {
+
+constexpr int kGateThreads = 256;
+constexpr int kGateMaxExperts = 1024;
+constexpr int kGateMaxK = 32;
+
+// ---------------------------------------------------------------- sort keys
+// Order-preserving integers: 0 for "not a candidate" (-inf or outside the row), the rest ascending with
+// the value, -0 equal to +0, every NaN above +inf.
+template <typename T>
+struct Key;
+
+template <typename T>
+struct Key16 {
+  using type = uint32_t;
+  __device__ static __forceinline__ type make(uint16_t bits, bool nan, int col) {
+    if (bits == 0x8000u) bits = 0;  // -0
+    uint32_t o = (bits & 0x8000u) ? static_cast<uint16_t>(~bits) : (bits | 0x8000u);
+    if (nan) o = 0xffffu;
+    return (o << 16) | static_cast<uint32_t>(0xffff - col);
+  }
+  __device__ static __forceinline__ uint16_t bits(type k) {
+    const uint32_t o = k >> 16;
+    return static_cast<uint16_t>((o & 0x8000u) ? (o & 0x7fffu) : ~o);
+  }
+  __device__ static __forceinline__ int col(type k) { return 0xffff - static_cast<int>(k & 0xffffu); }
+};
+template <>
+struct Key<__half> : Key16<__half> {
+  __device__ static __forceinline__ type of(__half v, int c) {
+    return __half2float(v) == -INFINITY ? 0u : make(__half_as_ushort(v), __hisnan(v), c);
+  }
+  __device__ static __forceinline__ float value(type k) { return __half2float(__ushort_as_half(bits(k))); }
+};
+template <>
+struct Key<__nv_bfloat16> : Key16<__nv_bfloat16> {
+  __device__ static __forceinline__ type of(__nv_bfloat16 v, int c) {
+    return __bfloat162float(v) == -INFINITY ? 0u : make(__bfloat16_as_ushort(v), __hisnan(v), c);
+  }
+  __device__ static __forceinline__ float value(type k) { return __bfloat162float(__ushort_as_bfloat16(bits(k))); }
+};
+template <>
+struct Key<float> {
+  using type = unsigned long long;
+  __device__ static __forceinline__ type of(float v, int c) {
+    if (v == -INFINITY) return 0ull;
+    uint32_t b = __float_as_uint(v);
+    if (b == 0x80000000u) b = 0;
+    uint32_t o = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+    if (isnan(v)) o = 0xffffffffu;
+    return (static_cast<type>(o) << 32) | static_cast<uint32_t>(0xffff - c);
+  }
+  __device__ static __forceinline__ float value(type k) {
+    const uint32_t o = static_cast<uint32_t>(k >> 32);
+    return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+  }
+  __device__ static __forceinline__ int col(type k) { return 0xffff - static_cast<int>(k & 0xffffu); }
+};
+template <>
+struct Key<double> {
+  using type = unsigned __int128;
+  __device__ static __forceinline__ type of(double v, int c) {
+    if (v == -INFINITY) return 0;
+    unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(v));
+    if (b == 0x8000000000000000ull) b = 0;
+    unsigned long long o = (b >> 63) ? ~b : (b | 0x8000000000000000ull);
+    if (isnan(v)) o = ~0ull;
+    return (static_cast<type>(o) << 64) | static_cast<unsigned long long>(0xffff - c);
+  }
+  __device__ static __forceinline__ double value(type k) {
+    const unsigned long long o = static_cast<unsigned long long>(k >> 64);
+    return __longlong_as_double(static_cast<long long>((o >> 63) ? (o & 0x7fffffffffffffffull) : ~o));
+  }
+  __device__ static __forceinline__ int col(type k) { return 0xffff - static_cast<int>(static_cast<uint32_t>(k) & 0xffffu); }
+};
+
+// Maximum over the 2^glog lanes of a group; every lane of the warp takes part.
+__device__ __forceinline__ uint32_t group_max(uint32_t v, int glog) {
+  if (glog == 5) return __reduce_max_sync(kFullMask, v);
+  for (int m = 1; m < (1 << glog); m <<= 1) v = max(v, __shfl_xor_sync(kFullMask, v, m));
+  return v;
+}
+__device__ __forceinline__ unsigned long long group_max(unsigned long long v, int glog) {
+  if (glog == 5) {
+    const uint32_t hi = static_cast<uint32_t>(v >> 32);
+    const uint32_t top = __reduce_max_sync(kFullMask, hi);
+    const uint32_t low = __reduce_max_sync(kFullMask, hi == top ? static_cast<uint32_t>(v) : 0u);
+    return (static_cast<unsigned long long>(top) << 32) | low;
+  }
+  for (int m = 1; m < (1 << glog); m <<= 1) {
+    const unsigned long long o = __shfl_xor_sync(kFullMask, v, m);
+    v = o > v ? o : v;
+  }
+  return v;
+}
+__device__ __forceinline__ unsigned __int128 group_max(unsigned __int128 v, int glog) {
+  for (int m = 1; m < (1 << glog); m <<= 1) {
+    const unsigned long long hi = __shfl_xor_sync(kFullMask, static_cast<unsigned long long>(v >> 64), m);
+    const unsigned long long lo = __shfl_xor_sync(kFullMask, static_cast<unsigned long long>(v), m);
+    const unsigned __int128 o = (static_cast<unsigned __int128>(hi) << 64) | lo;
+    v = o > v ? o : v;
+  }
+  return v;
+}
+
+// Column of a lane's i-th value: vectors of VE neighbouring columns, dealt to the lanes in turn.
+template <int VE>
+__device__ __forceinline__ int column(int i, int sub, int glog) {
+  return (((i / VE) << glog) + sub) * VE + i % VE;
+}
+
+// The row's values in the lane's registers, -inf outside the row.
+template <typename T, int V, int VE>
+__device__ __forceinline__ void load_row(const T* row, bool live, int E, int sub, int glog, T* v) {
+  const T none = from_acc<T>(-INFINITY);
+#pragma unroll
+  for (int i = 0; i < V; i += VE) {
+    const int c = column<VE>(i, sub, glog);
+    if (live && c < E) {  // E % VE == 0: a vector lies inside the row or outside it
+      const Raw<VE * sizeof(T)> r = ld_stream<VE * sizeof(T)>(row + c);
+      memcpy(v + i, &r, sizeof(r));
+    } else {
+#pragma unroll
+      for (int j = 0; j < VE; ++j) v[i + j] = none;
+    }
+  }
+}
+
+struct GateArgs {
+  const void* logits;
+  int64_t stride;
+  void* weights;
+  int32_t* experts;
+  int64_t N;
+  int E, k, glog;
+  bool renormalize;
+  const void* grad_weights;  // backward only
+  void* grad_logits;
+};
+
+template <typename T, int V, int VE>
+__global__ void __launch_bounds__(kGateThreads) gate_kernel(GateArgs a) {
+  using A = typename Acc<T>::type;
+  using K = typename Key<T>::type;
+  const int lane = threadIdx.x & 31, glog = a.glog, sub = lane & ((1 << glog) - 1);
+  const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kGateThreads >> 5) + (threadIdx.x >> 5);
+  const int64_t row = (warp << (5 - glog)) + (lane >> glog);
+  const bool live = row < a.N;
+  T v[V];
+  load_row<T, V, VE>(static_cast<const T*>(a.logits) + row * a.stride, live, a.E, sub, glog, v);
+  K key[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) key[i] = Key<T>::of(v[i], column<VE>(i, sub, glog));
+
+  K mine = 0;  // the s-th largest, in lane s of the group (k <= G)
+  A top = 0, sum = 0;
+  for (int s = 0; s < a.k; ++s) {
+    K m = key[0];
+#pragma unroll
+    for (int i = 1; i < V; ++i) m = key[i] > m ? key[i] : m;
+    m = group_max(m, glog);
+    if (s == 0) {
+      top = m ? Key<T>::value(m) : A(0);
+      if (!a.renormalize) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum += key[i] ? exp(to_acc<T>(v[i]) - top) : A(0);
+      }
+    }
+    if (sub == s) mine = m;
+#pragma unroll
+    for (int i = 0; i < V; ++i) key[i] = key[i] == m ? K(0) : key[i];
+  }
+  const A e = mine ? exp(Key<T>::value(mine) - top) : A(0);
+  if (a.renormalize) sum = e;
+  sum = group_sum(sum, glog);
+  if (live && sub < a.k) {
+    const int64_t at = row * a.k + sub;
+    a.experts[at] = mine ? Key<T>::col(mine) : -1;
+    static_cast<A*>(a.weights)[at] = mine ? e / sum : A(0);
+  }
+}
+
+// Gradient of the logits, with c = sum_s w_s g_s:
+//   renormalize: dl = w_s (g_s - c) on the chosen, 0 elsewhere;   otherwise: dl_j = p_j (g_j [chosen] - c).
+// The chosen columns' terms are put into a row of shared memory by the lane that holds the slot and read
+// back by the lane that owns the column.
+template <typename T, int V, int VE>
+__global__ void __launch_bounds__(kGateThreads) gate_backward_kernel(GateArgs a) {
+  using A = typename Acc<T>::type;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int lane = threadIdx.x & 31, glog = a.glog, sub = lane & ((1 << glog) - 1);
+  const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kGateThreads >> 5) + (threadIdx.x >> 5);
+  const int64_t row = (warp << (5 - glog)) + (lane >> glog);
+  const bool live = row < a.N;
+  A* term = reinterpret_cast<A*>(smem) + (static_cast<int>(threadIdx.x >> 5) * 32 + (lane - sub)) * V;
+#pragma unroll
+  for (int i = 0; i < V; ++i) term[column<VE>(i, sub, glog)] = A(0);
+
+  A w = 0, g = 0;
+  int col = -1;
+  if (live && sub < a.k) {
+    const int64_t at = row * a.k + sub;
+    col = a.experts[at];
+    if (col >= a.E) col = -1;
+    if (col >= 0) {
+      w = static_cast<const A*>(a.weights)[at];
+      g = static_cast<const A*>(a.grad_weights)[at];
+    }
+  }
+  const A c = group_sum(w * g, glog);
+  __syncwarp();
+  if (col >= 0) term[col] = a.renormalize ? w * (g - c) : g;
+  __syncwarp();
+
+  T* out = static_cast<T*>(a.grad_logits) + row * a.E;
+  A p[V];
+  if (!a.renormalize) {
+    T v[V];
+    load_row<T, V, VE>(static_cast<const T*>(a.logits) + row * a.stride, live, a.E, sub, glog, v);
+    A top = -INFINITY;
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      p[i] = to_acc<T>(v[i]);
+      top = p[i] > top ? p[i] : top;
+      nan |= isnan(p[i]);
+    }
+    for (int m = 1; m < (1 << glog); m <<= 1) {
+      const A o = __shfl_xor_sync(kFullMask, top, m);
+      top = o > top ? o : top;
+    }
+    const bool none = top == -INFINITY;
+    A sum = nan ? A(NAN) : A(0);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      p[i] = p[i] == -INFINITY ? A(0) : exp(p[i] - top);
+      sum += p[i];
+    }
+    sum = group_sum(sum, glog);
+#pragma unroll
+    for (int i = 0; i < V; ++i) p[i] = none && !isnan(sum) ? A(0) : p[i] / sum;
+  }
+#pragma unroll
+  for (int i = 0; i < V; i += VE) {
+    const int col0 = column<VE>(i, sub, glog);
+    if (!live || col0 >= a.E) continue;
+    A d[VE];
+#pragma unroll
+    for (int j = 0; j < VE; ++j) {
+      d[j] = term[col0 + j];
+      if (!a.renormalize) d[j] = p[i + j] * (d[j] - c);
+    }
+    st_row<VE * sizeof(T)>(out + col0, narrow<T, VE * sizeof(T)>(d));
+  }
+}
+
+template <typename T, int V, int VE>
+int launch_gate(const GateArgs& a, bool backward, cudaStream_t stream) {
+  const int64_t rows_per_block = static_cast<int64_t>(kGateThreads >> a.glog);
+  const int64_t blocks = (a.N + rows_per_block - 1) / rows_per_block;
+  if (blocks > 0x7fffffff) return fail(TBE_ERR_INVALID_ARGUMENT, "tbe_expert_gate: too many rows");
+  if (!backward) {
+    KernelTimer timer("gate_kernel", stream);
+    gate_kernel<T, V, VE><<<static_cast<unsigned>(blocks), kGateThreads, 0, stream>>>(a);
+  } else {
+    KernelTimer timer("gate_backward_kernel", stream);
+    const size_t shared = sizeof(typename Acc<T>::type) * kGateThreads * V;  // at most 64 KB (fp64, V = 32)
+    if (shared > 48 * 1024)
+      TBE_CUDA_TRY(cudaFuncSetAttribute(gate_backward_kernel<T, V, VE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        static_cast<int>(shared)));
+    gate_backward_kernel<T, V, VE><<<static_cast<unsigned>(blocks), kGateThreads, shared, stream>>>(a);
+  }
+  TBE_CHECK_LAUNCH(backward ? "gate_backward_kernel" : "gate_kernel");
+  return TBE_OK;
+}
+
+template <typename T, int VE>
+int launch_gate_width(const GateArgs& a, bool backward, cudaStream_t stream) {
+  const int per_lane = (a.E + (1 << a.glog) - 1) >> a.glog;
+  if (per_lane <= 8) return launch_gate<T, 8, VE>(a, backward, stream);
+  if (per_lane <= 16) return launch_gate<T, 16, VE>(a, backward, stream);
+  return launch_gate<T, 32, VE>(a, backward, stream);
+}
+
+template <typename T>
+int launch_gate_type(const GateArgs& a, bool backward, cudaStream_t stream) {
+  // 16-byte loads where every row starts on 16 bytes and ends on a vector; else one value at a time
+  constexpr int VE = 16 / sizeof(T);
+  const uint64_t bits = addr_bits(a.logits) | addr_bits(a.grad_logits) |
+                        (a.N > 1 ? static_cast<uint64_t>(a.stride) * sizeof(T) : 0);
+  if (bits % 16 == 0 && a.E % VE == 0) return launch_gate_width<T, VE>(a, backward, stream);
+  return launch_gate_width<T, 1>(a, backward, stream);
+}
+
+int run_gate(const char* who, GateArgs a, int dtype, bool backward, cudaStream_t stream) {
+  TBE_REQUIRE(a.N >= 0 && a.E > 0 && a.E <= kGateMaxExperts, "%s: the number of experts must be 1..%d", who,
+              kGateMaxExperts);
+  TBE_REQUIRE(a.k > 0 && a.k <= a.E && a.k <= kGateMaxK, "%s: k must be 1..min(E, %d)", who, kGateMaxK);
+  TBE_REQUIRE(known_dtype(dtype), "%s: bad dtype %d", who, dtype);
+  TBE_REQUIRE(a.N <= 1 || a.stride >= 0, "%s: negative row stride", who);
+  if (a.N == 0) return TBE_OK;
+  TBE_REQUIRE(a.logits && a.weights && a.experts, "%s: null pointer argument", who);
+  TBE_REQUIRE(!backward || (a.grad_weights && a.grad_logits), "%s: null pointer argument", who);
+  // lanes per row: eight values each (the narrowest group reads 16-bit rows as whole vectors), and a lane
+  // for every slot
+  a.glog = 0;
+  while (a.glog < 5 && ((8 << a.glog) < a.E || (1 << a.glog) < a.k)) ++a.glog;
+  switch (dtype) {
+    case TBE_F16: return launch_gate_type<__half>(a, backward, stream);
+    case TBE_BF16: return launch_gate_type<__nv_bfloat16>(a, backward, stream);
+    case TBE_F32: return launch_gate_type<float>(a, backward, stream);
+    default: return launch_gate_type<double>(a, backward, stream);
+  }
+}
+
+}  // namespace
+}  // namespace tbe
+
+extern "C" int tbe_expert_gate(const void* logits, int64_t row_stride, void* weights, int32_t* experts, int64_t N,
+                               int64_t E, int64_t k, int dtype, int renormalize, void* stream) {
+  using namespace tbe;
+  TBE_REQUIRE(E > 0 && E <= kGateMaxExperts && k > 0 && k <= kGateMaxK,
+              "tbe_expert_gate: E must be 1..%d and k 1..%d", kGateMaxExperts, kGateMaxK);
+  GateArgs a{logits, row_stride, weights, experts, N, static_cast<int>(E), static_cast<int>(k), 0, renormalize != 0,
+             nullptr, nullptr};
+  return run_gate("tbe_expert_gate", a, dtype, false, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int tbe_expert_gate_backward(const void* grad_weights, const void* logits, int64_t row_stride,
+                                        const void* weights, const int32_t* experts, void* grad_logits, int64_t N,
+                                        int64_t E, int64_t k, int dtype, int renormalize, void* stream) {
+  using namespace tbe;
+  TBE_REQUIRE(E > 0 && E <= kGateMaxExperts && k > 0 && k <= kGateMaxK,
+              "tbe_expert_gate_backward: E must be 1..%d and k 1..%d", kGateMaxExperts, kGateMaxK);
+  GateArgs a{logits, row_stride, const_cast<void*>(weights), const_cast<int32_t*>(experts), N, static_cast<int>(E),
+             static_cast<int>(k), 0, renormalize != 0, grad_weights, grad_logits};
+  return run_gate("tbe_expert_gate_backward", a, dtype, true, static_cast<cudaStream_t>(stream));
+}

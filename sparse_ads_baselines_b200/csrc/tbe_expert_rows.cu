@@ -1,0 +1,568 @@
+// Samples sorted by expert and back.
+//
+//   plan      experts[N][k] -> a stable counting sort of the M = N*k choices by expert:
+//             positions[t][s] = the row that choice (t, s) takes in expert order, order = its inverse,
+//             offsets[E+1] = where every expert's rows begin.  Choices outside 0..E-1 sort behind all
+//             experts; rows from offsets[E] ("kept") on belong to nobody.
+//   dispatch  y[positions[t][s]] = x[t];  rows behind kept are zero
+//   combine   out[t] = sum_s w[t][s] * y[positions[t][s]]   over the kept choices, slots ascending, fp32
+//             sums (fp64 for fp64), rounded once.  Without weights it is also dispatch's gradient.
+//   combine's gradient  dy[positions[t][s]] = w[t][s] * dout[t],  dw[t][s] = <dout[t], y[positions[t][s]]>
+//
+// Everything is indexed by sample, never by sorted row: a sample's row is read once and stored k times
+// (or k rows are read and one stored), so the traffic is the algorithm's, no sum needs an atomic and the
+// results do not depend on the order of anything.  All of it is bound by HBM.  A position outside the
+// rows is skipped by every kernel, so a wrong plan cannot reach memory outside the tensors.
+#include "tbe_elem.cuh"
+
+namespace tbe {
+namespace {
+
+constexpr int kMaxExperts = 1024;
+constexpr int kPlanSlice = 8192;  // choices per CTA of the two-kernel plan, at least
+
+// ---------------------------------------------------------------- plan
+struct PlanArgs {
+  const int32_t* experts;
+  int32_t* offsets;
+  int32_t* positions;
+  int32_t* order;
+  int32_t* counts;  // [ctas][E+1], two-kernel plan only
+  int32_t M, E, slice;
+};
+
+__device__ __forceinline__ int bin_of(int32_t id, int E) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(E) ? id : E; }
+
+// Exclusive prefix sum of v[0..n) in shared memory, by the whole CTA; n <= kMaxExperts + 1.
+__device__ void block_exclusive_scan(int32_t* v, int n, int32_t* warp_sums) {
+  const int per = (n + blockDim.x - 1) / blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int begin = min(static_cast<int>(threadIdx.x) * per, n), end = min(begin + per, n);
+  int32_t own = 0;
+  for (int i = begin; i < end; ++i) own += v[i];
+  int32_t scan = own;
+  for (int m = 1; m < 32; m <<= 1) {
+    const int32_t o = __shfl_up_sync(kFullMask, scan, m);
+    if (lane >= m) scan += o;
+  }
+  if (lane == 31) warp_sums[warp] = scan;
+  __syncthreads();
+  int32_t before = scan - own;
+  for (int w = 0; w < warp; ++w) before += warp_sums[w];
+  for (int i = begin; i < end; ++i) {
+    const int32_t x = v[i];
+    v[i] = before;
+    before += x;
+  }
+  __syncthreads();
+}
+
+// One CTA sorts its slice: every warp counts a contiguous part per bin, the parts are prefix-summed warp
+// by warp, and a second pass in the same order places each choice behind the earlier ones of its bin.
+// The order is therefore the stable one, whatever the atomics of the counting did.
+//   shared: hist[warps][E+1], start[E+1], before[E+1], 32 words
+template <bool MULTI>
+__global__ void __launch_bounds__(1024) plan_place_kernel(PlanArgs a) {
+  extern __shared__ int32_t plan_smem[];
+  const int E1 = a.E + 1, warps = blockDim.x >> 5, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int32_t* hist = plan_smem;
+  int32_t* start = hist + warps * E1;
+  int32_t* before = start + E1;
+  int32_t* warp_sums = before + E1;
+  const int64_t s0 = static_cast<int64_t>(blockIdx.x) * a.slice;
+  const int begin = static_cast<int>(s0 < a.M ? s0 : a.M), len = min(a.slice, a.M - begin);
+  const int part = ((len + warps - 1) / warps + 31) & ~31;
+  const int wb = begin + min(warp * part, len), we = begin + min((warp + 1) * part, len);
+
+  for (int i = threadIdx.x; i < warps * E1 + 2 * E1; i += blockDim.x) hist[i] = 0;
+  __syncthreads();
+  for (int i = wb + lane; i < we; i += 32) atomicAdd(&hist[warp * E1 + bin_of(__ldg(a.experts + i), a.E)], 1);
+  if (MULTI) {  // totals of every bin, and what the CTAs in front of this one put there
+    const int n = gridDim.x * E1, mine = blockIdx.x * E1;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const int32_t c = __ldg(a.counts + i);
+      const int b = i % E1;
+      if (c) {
+        atomicAdd(&start[b], c);
+        if (i < mine) atomicAdd(&before[b], c);
+      }
+    }
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < E1; b += blockDim.x) {
+    int32_t run = MULTI ? before[b] : 0;
+    for (int w = 0; w < warps; ++w) {
+      const int32_t c = hist[w * E1 + b];
+      hist[w * E1 + b] = run;
+      run += c;
+    }
+    if (!MULTI) start[b] = run;
+  }
+  __syncthreads();
+  block_exclusive_scan(start, E1, warp_sums);
+  if (blockIdx.x == 0)
+    for (int b = threadIdx.x; b < E1; b += blockDim.x) a.offsets[b] = start[b];
+
+  int32_t* next = hist + warp * E1;
+  for (int i0 = wb; i0 < we; i0 += 32) {
+    const int i = i0 + lane;
+    const bool on = i < we;
+    const int b = on ? bin_of(__ldg(a.experts + i), a.E) : E1;
+    const unsigned peers = __match_any_sync(kFullMask, b);
+    const int rank = __popc(peers & ((1u << lane) - 1));
+    const int32_t first = on ? next[b] : 0;
+    __syncwarp();
+    if (on && rank == 0) next[b] = first + __popc(peers);
+    __syncwarp();
+    if (on) {
+      const int32_t p = start[b] + first + rank;
+      a.positions[i] = p;
+      a.order[p] = i;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(1024) plan_count_kernel(PlanArgs a) {
+  extern __shared__ int32_t plan_smem[];
+  const int E1 = a.E + 1;
+  const int64_t s0 = static_cast<int64_t>(blockIdx.x) * a.slice;
+  const int begin = static_cast<int>(s0 < a.M ? s0 : a.M), end = begin + min(a.slice, a.M - begin);
+  for (int b = threadIdx.x; b < E1; b += blockDim.x) plan_smem[b] = 0;
+  __syncthreads();
+  for (int i = begin + threadIdx.x; i < end; i += blockDim.x) atomicAdd(&plan_smem[bin_of(__ldg(a.experts + i), a.E)], 1);
+  __syncthreads();
+  for (int b = threadIdx.x; b < E1; b += blockDim.x) a.counts[static_cast<int64_t>(blockIdx.x) * E1 + b] = plan_smem[b];
+}
+
+struct PlanShape {
+  int ctas, slice;
+};
+PlanShape plan_shape(int64_t M) {
+  int64_t ctas = (M + kPlanSlice - 1) / kPlanSlice;
+  if (ctas > 148) ctas = 148;
+  if (ctas < 1) ctas = 1;
+  return {static_cast<int>(ctas), static_cast<int>((M + ctas - 1) / ctas)};
+}
+
+// ---------------------------------------------------------------- rows
+struct RowArgs {
+  const char* x;       // dispatch: rows by sample; combine: rows by position
+  int64_t x_stride;    // bytes
+  const int32_t* positions;
+  const int32_t* kept;  // offsets + E
+  const void* weights;  // [N][k] in the accumulator type, or NULL
+  char* out;
+  int64_t row_bytes;  // stride of position-ordered and freshly written rows
+  int32_t M;
+  int k;
+  uint32_t nvec, items;  // vectors per row, (sample, vector) pairs of this launch
+  FastDiv div;           // by nvec
+};
+
+__device__ __forceinline__ uint32_t kept_rows(const int32_t* kept, int32_t M) {
+  const int32_t n = __ldg(kept);
+  return static_cast<uint32_t>(n < 0 ? 0 : n > M ? M : n);
+}
+
+// A thread takes U (sample, vector) pairs a CTA width apart: U independent loads, then k stores each.
+template <int VB, int U>
+__global__ void __launch_bounds__(256) dispatch_kernel(RowArgs a) {
+  const uint32_t base = blockIdx.x * (256u * U) + threadIdx.x;
+  Raw<VB> r[U];
+  uint32_t t[U], v[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t i = base + u * 256u;
+    t[u] = fastdiv(i, a.div);
+    v[u] = (i - t[u] * a.nvec) * VB;
+    if (i < a.items) r[u] = ld_stream<VB>(a.x + t[u] * a.x_stride + v[u]);
+  }
+  const uint32_t kept = kept_rows(a.kept, a.M), M = static_cast<uint32_t>(a.M);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (base + u * 256u >= a.items) break;
+    const int32_t* pos = a.positions + static_cast<int64_t>(t[u]) * a.k;
+    for (int s = 0; s < a.k; ++s) {
+      const uint32_t p = static_cast<uint32_t>(__ldg(pos + s));
+      if (p < M) st_row<VB>(a.out + p * a.row_bytes + v[u], p < kept ? r[u] : raw_none<VB>());
+    }
+  }
+}
+
+// A thread sums one vector of a sample's row; KB row loads are in flight together.
+template <typename T, int VB, int KB>
+__global__ void __launch_bounds__(256) combine_kernel(RowArgs a) {
+  using A = typename Acc<T>::type;
+  constexpr int NE = VB / sizeof(T);
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+  if (i >= a.items) return;
+  const uint32_t t = fastdiv(i, a.div), v = (i - t * a.nvec) * VB;
+  const int64_t at = static_cast<int64_t>(t) * a.k;
+  const uint32_t kept = kept_rows(a.kept, a.M);
+  A acc[NE];
+#pragma unroll
+  for (int e = 0; e < NE; ++e) acc[e] = A(0);
+  for (int s0 = 0; s0 < a.k; s0 += KB) {
+    Raw<VB> r[KB];
+    bool in[KB];
+    A w[KB];
+#pragma unroll
+    for (int s = 0; s < KB; ++s) {
+      const bool on = s0 + s < a.k;
+      const uint32_t p = on ? static_cast<uint32_t>(__ldg(a.positions + at + s0 + s)) : 0xffffffffu;
+      in[s] = p < kept;
+      w[s] = in[s] && a.weights ? __ldg(static_cast<const A*>(a.weights) + at + s0 + s) : A(1);
+      if (in[s]) r[s] = ld_stream<VB>(a.x + p * a.x_stride + v);
+    }
+#pragma unroll
+    for (int s = 0; s < KB; ++s) {
+      if (!in[s]) continue;
+      A e[NE];
+      expand<T, VB>(r[s], e);
+#pragma unroll
+      for (int j = 0; j < NE; ++j) acc[j] += w[s] * e[j];
+    }
+  }
+  st_row<VB>(a.out + t * a.row_bytes + v, narrow<T, VB>(acc));
+}
+
+struct GradArgs {
+  const char* grad_out;  // [N], row stride go_stride bytes
+  int64_t go_stride;
+  const char* y;
+  const int32_t* positions;
+  const int32_t* kept;
+  const void* weights;
+  char* grad_y;        // or NULL
+  void* grad_weights;  // or NULL
+  int64_t row_bytes;
+  int64_t N;
+  int32_t M;
+  int k;
+  int nvec;
+};
+
+// G lanes per sample walk its row: the upstream row is held in registers while KB expert rows are read
+// against it (dot products) and KB scaled copies are stored.
+template <typename T, int VB, int G, int KB>
+__global__ void __launch_bounds__(G == 128 ? 128 : 256) combine_backward_kernel(GradArgs a) {
+  using A = typename Acc<T>::type;
+  constexpr int NE = VB / sizeof(T), kThreads = G == 128 ? 128 : 256;
+  __shared__ A part[4][KB];
+  const int sub = threadIdx.x % G;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * (kThreads / G) + threadIdx.x / G;
+  const bool live = t < a.N;
+  const uint32_t kept = kept_rows(a.kept, a.M), M = static_cast<uint32_t>(a.M);
+  const char* go = a.grad_out + (live ? t : 0) * a.go_stride;
+  for (int s0 = 0; s0 < a.k; s0 += KB) {
+    uint32_t p[KB];
+    A w[KB], dot[KB];
+#pragma unroll
+    for (int s = 0; s < KB; ++s) {
+      const bool on = live && s0 + s < a.k;
+      p[s] = on ? static_cast<uint32_t>(__ldg(a.positions + t * a.k + s0 + s)) : 0xffffffffu;
+      w[s] = on ? __ldg(static_cast<const A*>(a.weights) + t * a.k + s0 + s) : A(0);
+      dot[s] = A(0);
+    }
+    for (int v = live ? sub : a.nvec; v < a.nvec; v += G) {
+      const int64_t off = static_cast<int64_t>(v) * VB;
+      const Raw<VB> gr = ld_stream<VB>(go + off);
+      Raw<VB> r[KB];
+      if (a.grad_weights) {
+#pragma unroll
+        for (int s = 0; s < KB; ++s)
+          if (p[s] < kept) r[s] = ld_stream<VB>(a.y + p[s] * a.row_bytes + off);
+      }
+      A g[NE];
+      expand<T, VB>(gr, g);
+#pragma unroll
+      for (int s = 0; s < KB; ++s) {
+        if (a.grad_weights && p[s] < kept) {
+          A e[NE];
+          expand<T, VB>(r[s], e);
+#pragma unroll
+          for (int j = 0; j < NE; ++j) dot[s] += g[j] * e[j];
+        }
+        if (a.grad_y && p[s] < M) {
+          A d[NE];
+#pragma unroll
+          for (int j = 0; j < NE; ++j) d[j] = p[s] < kept ? w[s] * g[j] : A(0);
+          st_row<VB>(a.grad_y + p[s] * a.row_bytes + off, narrow<T, VB>(d));
+        }
+      }
+    }
+    if (a.grad_weights) {
+#pragma unroll
+      for (int s = 0; s < KB; ++s)
+#pragma unroll
+        for (int m = 1; m < (G < 32 ? G : 32); m <<= 1) dot[s] += __shfl_xor_sync(kFullMask, dot[s], m);
+      if (G == 128) {
+        if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+          for (int s = 0; s < KB; ++s) part[threadIdx.x >> 5][s] = dot[s];
+        }
+        __syncthreads();
+        if (threadIdx.x < KB && s0 + static_cast<int>(threadIdx.x) < a.k)
+          static_cast<A*>(a.grad_weights)[t * a.k + s0 + threadIdx.x] =
+              (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
+        __syncthreads();
+      } else if (live && sub == 0) {
+#pragma unroll
+        for (int s = 0; s < KB; ++s)
+          if (s0 + s < a.k) static_cast<A*>(a.grad_weights)[t * a.k + s0 + s] = dot[s];
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- launches
+// 32-bit pair indices: a launch covers as many samples as fit below 2^32 pairs.
+int64_t rows_per_launch(int64_t nvec) {
+  const int64_t n = (0xffffffffll - 4096) / nvec;
+  return n < 1 ? 1 : n;
+}
+
+template <int VB>
+int launch_dispatch(RowArgs a, int64_t N, cudaStream_t stream) {
+  constexpr int U = 2;
+  a.nvec = static_cast<uint32_t>(a.row_bytes / VB);
+  a.div = make_fastdiv(a.nvec);
+  const int64_t step = rows_per_launch(a.nvec);
+  for (int64_t n0 = 0; n0 < N; n0 += step) {
+    RowArgs b = a;
+    const int64_t n = N - n0 < step ? N - n0 : step;
+    b.x = a.x + n0 * a.x_stride;
+    b.positions = a.positions + n0 * a.k;
+    b.items = static_cast<uint32_t>(n * a.nvec);
+    const uint32_t blocks = static_cast<uint32_t>((static_cast<int64_t>(b.items) + 256 * U - 1) / (256 * U));
+    {
+      KernelTimer timer("dispatch_kernel", stream);
+      dispatch_kernel<VB, U><<<blocks, 256, 0, stream>>>(b);
+    }
+    TBE_CHECK_LAUNCH("dispatch_kernel");
+  }
+  return TBE_OK;
+}
+
+template <typename T, int VB, int KB>
+int launch_combine_k(RowArgs a, int64_t N, cudaStream_t stream) {
+  using A = typename Acc<T>::type;
+  a.nvec = static_cast<uint32_t>(a.row_bytes / VB);
+  a.div = make_fastdiv(a.nvec);
+  const int64_t step = rows_per_launch(a.nvec);
+  for (int64_t n0 = 0; n0 < N; n0 += step) {
+    RowArgs b = a;
+    const int64_t n = N - n0 < step ? N - n0 : step;
+    b.positions = a.positions + n0 * a.k;
+    b.weights = a.weights ? static_cast<const A*>(a.weights) + n0 * a.k : nullptr;
+    b.out = a.out + n0 * a.row_bytes;
+    b.items = static_cast<uint32_t>(n * a.nvec);
+    const uint32_t blocks = static_cast<uint32_t>((static_cast<int64_t>(b.items) + 255) / 256);
+    {
+      KernelTimer timer("combine_kernel", stream);
+      combine_kernel<T, VB, KB><<<blocks, 256, 0, stream>>>(b);
+    }
+    TBE_CHECK_LAUNCH("combine_kernel");
+  }
+  return TBE_OK;
+}
+
+template <typename T, int VB>
+int launch_combine(const RowArgs& a, int64_t N, cudaStream_t stream) {
+  if constexpr (VB < static_cast<int>(sizeof(T))) {
+    return fail(TBE_ERR_INVALID_ARGUMENT, "tbe_expert_combine: rows must be aligned to their element size");
+  } else {
+    if (a.k <= 2) return launch_combine_k<T, VB, 2>(a, N, stream);
+    if (a.k <= 4) return launch_combine_k<T, VB, 4>(a, N, stream);
+    return launch_combine_k<T, VB, 8>(a, N, stream);
+  }
+}
+
+template <typename T>
+int launch_combine_type(const RowArgs& a, int vb, int64_t N, cudaStream_t stream) {
+  switch (vb) {
+    case 16: return launch_combine<T, 16>(a, N, stream);
+    case 8: return launch_combine<T, 8>(a, N, stream);
+    case 4: return launch_combine<T, 4>(a, N, stream);
+    default: return launch_combine<T, 2>(a, N, stream);
+  }
+}
+
+template <typename T, int VB, int G, int KB>
+int launch_backward_gk(const GradArgs& a, cudaStream_t stream) {
+  constexpr int kThreads = G == 128 ? 128 : 256;
+  const int64_t blocks = (a.N + kThreads / G - 1) / (kThreads / G);
+  {
+    KernelTimer timer("combine_backward_kernel", stream);
+    combine_backward_kernel<T, VB, G, KB><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(a);
+  }
+  TBE_CHECK_LAUNCH("combine_backward_kernel");
+  return TBE_OK;
+}
+
+template <typename T, int VB, int G>
+int launch_backward_g(const GradArgs& a, cudaStream_t stream) {
+  if (a.k <= 2) return launch_backward_gk<T, VB, G, 2>(a, stream);
+  if (a.k <= 4) return launch_backward_gk<T, VB, G, 4>(a, stream);
+  return launch_backward_gk<T, VB, G, 8>(a, stream);
+}
+
+template <typename T, int VB>
+int launch_backward(GradArgs a, cudaStream_t stream) {
+  if constexpr (VB < static_cast<int>(sizeof(T))) {
+    return fail(TBE_ERR_INVALID_ARGUMENT, "tbe_expert_combine_backward: rows must be aligned to their element size");
+  } else {
+    a.nvec = static_cast<int>(a.row_bytes / VB);
+    if (a.nvec <= 16) return launch_backward_g<T, VB, 8>(a, stream);
+    if (a.nvec <= 96) return launch_backward_g<T, VB, 32>(a, stream);
+    return launch_backward_g<T, VB, 128>(a, stream);
+  }
+}
+
+template <typename T>
+int launch_backward_type(const GradArgs& a, int vb, cudaStream_t stream) {
+  switch (vb) {
+    case 16: return launch_backward<T, 16>(a, stream);
+    case 8: return launch_backward<T, 8>(a, stream);
+    case 4: return launch_backward<T, 4>(a, stream);
+    default: return launch_backward<T, 2>(a, stream);
+  }
+}
+
+int check_rows(const char* who, int64_t N, int64_t k, int64_t D, int dtype) {
+  TBE_REQUIRE(known_dtype(dtype), "%s: bad dtype %d", who, dtype);
+  TBE_REQUIRE(N >= 0 && k > 0 && D > 0 && N < (1ll << 31) && k < (1ll << 31) && N * k < (1ll << 31),
+              "%s: N must be >= 0, k and D > 0, and N*k < 2^31", who);
+  TBE_REQUIRE(D <= (1ll << 28), "%s: rows of more than 2^28 elements are not supported", who);
+  return TBE_OK;
+}
+
+}  // namespace
+}  // namespace tbe
+
+extern "C" int64_t tbe_expert_plan_workspace_bytes(int64_t M, int64_t E) {
+  using namespace tbe;
+  if (M < 0 || M >= (1ll << 31) || E < 1 || E > kMaxExperts)
+    return fail(TBE_ERR_INVALID_ARGUMENT, "tbe_expert_plan_workspace_bytes: M must be 0..2^31-1 and E 1..%d", kMaxExperts);
+  const PlanShape s = plan_shape(M);
+  return s.ctas == 1 ? 0 : static_cast<int64_t>(s.ctas) * (E + 1) * 4;
+}
+
+extern "C" int tbe_expert_plan(const int32_t* experts, int32_t* offsets, int32_t* positions, int32_t* order, int64_t M,
+                               int64_t E, void* workspace, int64_t workspace_bytes, void* stream_v) {
+  using namespace tbe;
+  const int64_t need = tbe_expert_plan_workspace_bytes(M, E);
+  if (need < 0) return static_cast<int>(need);
+  TBE_REQUIRE(offsets && (M == 0 || (experts && positions && order)), "tbe_expert_plan: null pointer argument");
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(TBE_ERR_WORKSPACE_TOO_SMALL, "tbe_expert_plan: workspace of %lld bytes, %lld needed",
+                static_cast<long long>(workspace_bytes), static_cast<long long>(need));
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  const PlanShape s = plan_shape(M);
+  PlanArgs a{experts, offsets, positions, order, static_cast<int32_t*>(workspace), static_cast<int32_t>(M),
+             static_cast<int32_t>(E), s.slice};
+  const int threads = M <= 1024 ? 256 : 1024;
+  const size_t shared = (static_cast<size_t>(threads / 32 + 2) * (E + 1) + 32) * 4;
+  auto place = s.ctas == 1 ? plan_place_kernel<false> : plan_place_kernel<true>;
+  if (shared > 48 * 1024)
+    TBE_CUDA_TRY(cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)));
+  if (s.ctas > 1) {
+    {
+      KernelTimer timer("plan_count_kernel", stream);
+      plan_count_kernel<<<s.ctas, 1024, (E + 1) * 4, stream>>>(a);
+    }
+    TBE_CHECK_LAUNCH("plan_count_kernel");
+  }
+  {
+    KernelTimer timer("plan_place_kernel", stream);
+    place<<<s.ctas, threads, shared, stream>>>(a);
+  }
+  TBE_CHECK_LAUNCH("plan_place_kernel");
+  return TBE_OK;
+}
+
+extern "C" int tbe_expert_dispatch(const void* x, int64_t row_stride, const int32_t* positions, const int32_t* offsets,
+                                   void* y, int64_t N, int64_t k, int64_t D, int64_t E, int dtype, void* stream_v) {
+  using namespace tbe;
+  if (const int rc = check_rows("tbe_expert_dispatch", N, k, D, dtype)) return rc;
+  if (N == 0) return TBE_OK;
+  TBE_REQUIRE(x && positions && offsets && y, "tbe_expert_dispatch: null pointer argument");
+  TBE_REQUIRE(E > 0 && (N == 1 || row_stride >= 0), "tbe_expert_dispatch: E must be > 0, row_stride >= 0");
+  const int64_t es = any_elem_size(dtype);
+  RowArgs a{};
+  a.x = static_cast<const char*>(x);
+  a.x_stride = N == 1 ? 0 : row_stride * es;
+  a.positions = positions;
+  a.kept = offsets + E;
+  a.out = static_cast<char*>(y);
+  a.row_bytes = D * es;
+  a.M = static_cast<int32_t>(N * k);
+  a.k = static_cast<int>(k);
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  switch (vector_bytes_of(addr_bits(x) | addr_bits(y) | static_cast<uint64_t>(a.x_stride) | static_cast<uint64_t>(a.row_bytes))) {
+    case 16: return launch_dispatch<16>(a, N, stream);
+    case 8: return launch_dispatch<8>(a, N, stream);
+    case 4: return launch_dispatch<4>(a, N, stream);
+    default: return launch_dispatch<2>(a, N, stream);
+  }
+}
+
+extern "C" int tbe_expert_combine(const void* y, const int32_t* positions, const int32_t* offsets, const void* weights,
+                                  void* out, int64_t N, int64_t k, int64_t D, int64_t E, int dtype, void* stream_v) {
+  using namespace tbe;
+  if (const int rc = check_rows("tbe_expert_combine", N, k, D, dtype)) return rc;
+  if (N == 0) return TBE_OK;
+  TBE_REQUIRE(y && positions && offsets && out, "tbe_expert_combine: null pointer argument");
+  TBE_REQUIRE(E > 0, "tbe_expert_combine: E must be > 0");
+  RowArgs a{};
+  a.x = static_cast<const char*>(y);
+  a.row_bytes = a.x_stride = D * any_elem_size(dtype);
+  a.positions = positions;
+  a.kept = offsets + E;
+  a.weights = weights;
+  a.out = static_cast<char*>(out);
+  a.M = static_cast<int32_t>(N * k);
+  a.k = static_cast<int>(k);
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  const int vb = vector_bytes_of(addr_bits(y) | addr_bits(out) | static_cast<uint64_t>(a.row_bytes));
+  switch (dtype) {
+    case TBE_F16: return launch_combine_type<__half>(a, vb, N, stream);
+    case TBE_BF16: return launch_combine_type<__nv_bfloat16>(a, vb, N, stream);
+    case TBE_F32: return launch_combine_type<float>(a, vb, N, stream);
+    default: return launch_combine_type<double>(a, vb, N, stream);
+  }
+}
+
+extern "C" int tbe_expert_combine_backward(const void* grad_out, int64_t grad_stride, const void* y,
+                                           const int32_t* positions, const int32_t* offsets, const void* weights,
+                                           void* grad_y, void* grad_weights, int64_t N, int64_t k, int64_t D, int64_t E,
+                                           int dtype, void* stream_v) {
+  using namespace tbe;
+  if (const int rc = check_rows("tbe_expert_combine_backward", N, k, D, dtype)) return rc;
+  if (N == 0 || (!grad_y && !grad_weights)) return TBE_OK;
+  TBE_REQUIRE(grad_out && positions && offsets && weights && (y || !grad_weights),
+              "tbe_expert_combine_backward: null pointer argument");
+  TBE_REQUIRE(E > 0 && (N == 1 || grad_stride >= 0), "tbe_expert_combine_backward: E must be > 0, grad_stride >= 0");
+  const int64_t es = any_elem_size(dtype);
+  GradArgs a{};
+  a.grad_out = static_cast<const char*>(grad_out);
+  a.go_stride = N == 1 ? 0 : grad_stride * es;
+  a.y = static_cast<const char*>(y);
+  a.positions = positions;
+  a.kept = offsets + E;
+  a.weights = weights;
+  a.grad_y = static_cast<char*>(grad_y);
+  a.grad_weights = grad_weights;
+  a.row_bytes = D * es;
+  a.N = N;
+  a.M = static_cast<int32_t>(N * k);
+  a.k = static_cast<int>(k);
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  const int vb = vector_bytes_of(addr_bits(grad_out) | addr_bits(y) | addr_bits(grad_y) |
+                                 static_cast<uint64_t>(a.go_stride) | static_cast<uint64_t>(a.row_bytes));
+  switch (dtype) {
+    case TBE_F16: return launch_backward_type<__half>(a, vb, stream);
+    case TBE_BF16: return launch_backward_type<__nv_bfloat16>(a, vb, stream);
+    case TBE_F32: return launch_backward_type<float>(a, vb, stream);
+    default: return launch_backward_type<double>(a, vb, stream);
+  }
+}

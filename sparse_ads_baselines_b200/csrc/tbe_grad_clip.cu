@@ -1,0 +1,379 @@
+// The 2-norm over a list of gradients, and the gradients scaled down to a largest norm.
+//
+//   n = sqrt(sum over all tensors of g^2);   c = min(1, max_norm / (n + eps));   g <- c * g
+//
+// A list is cut into chunks of kChunk elements, dealt to a grid that fills the GPU; every CTA sums its
+// chunks' squares in fp64 into one partial, and the kernel that needs the norm adds the partials in their
+// order, so the result is the same from run to run and no counter has to be cleared between calls.  The
+// table of tensors travels in the kernel's parameters: no copy to the device, nothing to keep alive, and
+// a captured graph holds it.  Lists that are too long for one launch take several.
+//
+// Bound by HBM.  The norm has to be known before the first element is scaled, so a list larger than L2 is
+// read twice; the scaling pass runs through the chunks backwards, so that what the norm pass read last is
+// still in L2.  In place and with c == 1 there is nothing to store and the second pass ends at once.
+#include <algorithm>
+#include <new>
+
+#include "tbe_elem.cuh"
+
+namespace tbe {
+namespace {
+
+constexpr int kClipThreads = 256;
+constexpr int kClipBlocksPerSM = 8;
+constexpr int kChunk = 16384;      // elements
+constexpr int kSmallTable = 64;    // tensors whose table fits a small parameter block
+constexpr int kLargeTable = 1024;  // and the largest (30 KB of parameters)
+
+template <int CAP>
+struct Table {
+  const void* src[CAP];
+  void* dst[CAP];
+  int64_t n[CAP];
+  int32_t first[CAP];  // first chunk of the tensor
+  uint8_t dtype[CAP];
+  int32_t count, chunks;
+};
+
+template <int CAP>
+__device__ __forceinline__ int tensor_of(const Table<CAP>& t, int chunk) {
+  int lo = 0, hi = t.count;  // first[lo] <= chunk < first[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (t.first[mid] <= chunk) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Sum of the squares of a vector.  fp32 and fp64 values are squared in fp64.  Sixteen-bit values are
+// squared and summed over the vector in fp32 (eight terms, relative error 2^-21) unless a square leaves
+// fp32's range, which only bfloat16 reaches; then in fp64 too.
+template <typename T, int VB>
+__device__ __forceinline__ double sum_squares(const Raw<VB>& r) {
+  constexpr int N = VB / sizeof(T);
+  typename Acc<T>::type e[N];
+  expand<T, VB>(r, e);
+  if constexpr (sizeof(T) == 2) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) s += e[i] * e[i];
+    // in the range [1e-24, 1e38] no term that counts has lost digits; NaN and inf take the slow way and stay
+    if (s >= 1e-24f && s <= 1e38f) return s;
+  }
+  double d = 0.0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) d += static_cast<double>(e[i]) * static_cast<double>(e[i]);
+  return d;
+}
+
+template <typename T>
+__device__ double chunk_squares(const T* p, int n) {
+  constexpr int NV = 16 / sizeof(T), U = 4;
+  const int head = min(n, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / static_cast<int>(sizeof(T)));
+  const int nvec = (n - head) / NV, tail = head + nvec * NV;
+  double s = 0.0;
+  for (int i = threadIdx.x; i < head; i += kClipThreads) s += sum_squares<T, sizeof(T)>(ld_stream<sizeof(T)>(p + i));
+  for (int i = tail + threadIdx.x; i < n; i += kClipThreads) s += sum_squares<T, sizeof(T)>(ld_stream<sizeof(T)>(p + i));
+  const T* q = p + head;
+  for (int v = threadIdx.x; v < nvec; v += kClipThreads * U) {
+    Raw<16> r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = v + u * kClipThreads;
+      r[u] = i < nvec ? ld_stream<16>(q + static_cast<int64_t>(i) * NV) : raw_none<16>();
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) s += sum_squares<T, 16>(r[u]);
+  }
+  return s;
+}
+
+// Sum over the CTA in a fixed order; every thread gets it.
+__device__ __forceinline__ double block_sum(double v) {
+  __shared__ double part[kClipThreads / 32];
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) v += __shfl_xor_sync(kFullMask, v, m);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double s = 0.0;
+#pragma unroll
+  for (int w = 0; w < kClipThreads / 32; ++w) s += part[w];
+  __syncthreads();
+  return s;
+}
+
+template <int CAP>
+__global__ void __launch_bounds__(kClipThreads) grad_norm_kernel(const __grid_constant__ Table<CAP> t, double* partial) {
+  double s = 0.0;
+  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+    const int k = tensor_of(t, c);
+    const int64_t at = static_cast<int64_t>(c - t.first[k]) * kChunk;
+    const int64_t left = t.n[k] - at;
+    const int n = static_cast<int>(left < kChunk ? left : kChunk);
+    switch (t.dtype[k]) {
+      case TBE_F16: s += chunk_squares(static_cast<const __half*>(t.src[k]) + at, n); break;
+      case TBE_BF16: s += chunk_squares(static_cast<const __nv_bfloat16*>(t.src[k]) + at, n); break;
+      case TBE_F32: s += chunk_squares(static_cast<const float*>(t.src[k]) + at, n); break;
+      default: s += chunk_squares(static_cast<const double*>(t.src[k]) + at, n); break;
+    }
+  }
+  s = block_sum(s);
+  if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+
+__device__ __forceinline__ double fold(const double* partial, int n) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += kClipThreads) s += partial[i];
+  return sqrt(block_sum(s));
+}
+
+__global__ void __launch_bounds__(kClipThreads) grad_norm_finish_kernel(const double* partial, int n, float* norm) {
+  const double r = fold(partial, n);
+  if (threadIdx.x == 0) *norm = static_cast<float>(r);
+}
+
+template <typename T>
+__device__ void scale_chunk(const T* src, T* dst, int n, double c) {
+  using A = typename Acc<T>::type;
+  constexpr int NV = 16 / sizeof(T), U = 4;
+  const A f = static_cast<A>(c);
+  const uintptr_t s = reinterpret_cast<uintptr_t>(src), d = reinterpret_cast<uintptr_t>(dst);
+  int head = min(n, static_cast<int>((16 - (s & 15)) & 15) / static_cast<int>(sizeof(T)));
+  int nvec = (n - head) / NV;
+  if ((s ^ d) & 15) {  // no vector of one is a vector of the other
+    head = n;
+    nvec = 0;
+  }
+  const int tail = head + nvec * NV;
+  for (int i = threadIdx.x; i < head; i += kClipThreads) dst[i] = from_acc<T>(to_acc<T>(src[i]) * f);
+  for (int i = tail + threadIdx.x; i < n; i += kClipThreads) dst[i] = from_acc<T>(to_acc<T>(src[i]) * f);
+  for (int v = threadIdx.x; v < nvec; v += kClipThreads * U) {
+    Raw<16> r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = v + u * kClipThreads;
+      if (i < nvec) r[u] = ld_rw<16>(src + head + static_cast<int64_t>(i) * NV);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = v + u * kClipThreads;
+      if (i < nvec) {
+        A e[NV];
+        expand<T, 16>(r[u], e);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) e[j] *= f;
+        st_row<16>(dst + head + static_cast<int64_t>(i) * NV, narrow<T, 16>(e));
+      }
+    }
+  }
+}
+
+template <int CAP>
+__global__ void __launch_bounds__(kClipThreads) grad_scale_kernel(const __grid_constant__ Table<CAP> t, const double* partial,
+                                                                  int parts, double max_norm, double eps, bool in_place,
+                                                                  float* norm) {
+  const double n2 = fold(partial, parts);
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n2);
+  double f = max_norm / (n2 + eps);
+  if (f > 1.0) f = 1.0;  // NaN stays
+  if (in_place && f == 1.0) return;
+  for (int c = t.chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {
+    const int k = tensor_of(t, c);
+    const int64_t at = static_cast<int64_t>(c - t.first[k]) * kChunk;
+    const int64_t left = t.n[k] - at;
+    const int n = static_cast<int>(left < kChunk ? left : kChunk);
+    switch (t.dtype[k]) {
+      case TBE_F16: scale_chunk(static_cast<const __half*>(t.src[k]) + at, static_cast<__half*>(t.dst[k]) + at, n, f); break;
+      case TBE_BF16:
+        scale_chunk(static_cast<const __nv_bfloat16*>(t.src[k]) + at, static_cast<__nv_bfloat16*>(t.dst[k]) + at, n, f);
+        break;
+      case TBE_F32: scale_chunk(static_cast<const float*>(t.src[k]) + at, static_cast<float*>(t.dst[k]) + at, n, f); break;
+      default: scale_chunk(static_cast<const double*>(t.src[k]) + at, static_cast<double*>(t.dst[k]) + at, n, f); break;
+    }
+  }
+}
+
+// One launch's worth of the list: tensors [from, to), at most CAP of them, empty ones left out.
+template <int CAP>
+bool fill(Table<CAP>& t, const void* const* src, void* const* dst, const int64_t* n, const int32_t* dtype, int from, int to) {
+  t.count = 0;
+  int64_t chunks = 0;
+  for (int i = from; i < to; ++i) {
+    if (n[i] == 0) continue;
+    t.src[t.count] = src[i];
+    t.dst[t.count] = dst ? dst[i] : nullptr;
+    t.n[t.count] = n[i];
+    t.first[t.count] = static_cast<int32_t>(chunks);
+    t.dtype[t.count] = static_cast<uint8_t>(dtype[i]);
+    ++t.count;
+    chunks += (n[i] + kChunk - 1) / kChunk;
+    if (chunks > 0x7fff0000) return false;
+  }
+  t.chunks = static_cast<int32_t>(chunks);
+  return true;
+}
+
+int launch_grid(int64_t chunks) {
+  const int64_t most = static_cast<int64_t>(device_sm_count()) * kClipBlocksPerSM;
+  return static_cast<int>(chunks < most ? (chunks > 0 ? chunks : 1) : most);
+}
+
+int check_list(const char* who, const void* const* src, const int64_t* n, const int32_t* dtype, int64_t count) {
+  TBE_REQUIRE(count >= 0 && count < (1ll << 24), "%s: the number of tensors must be 0..2^24-1", who);
+  TBE_REQUIRE(count == 0 || (src && n && dtype), "%s: null pointer argument", who);
+  for (int64_t i = 0; i < count; ++i) {
+    TBE_REQUIRE(known_dtype(dtype[i]), "%s: tensor %lld has bad dtype %d", who, static_cast<long long>(i), dtype[i]);
+    TBE_REQUIRE(n[i] >= 0 && n[i] < (1ll << 44), "%s: tensor %lld has a bad size", who, static_cast<long long>(i));
+    TBE_REQUIRE(n[i] == 0 || src[i], "%s: tensor %lld is a null pointer", who, static_cast<long long>(i));
+    TBE_REQUIRE(addr_bits(src[i]) % any_elem_size(dtype[i]) == 0, "%s: tensor %lld is not aligned to its elements", who,
+                static_cast<long long>(i));
+  }
+  return TBE_OK;
+}
+
+// Stores of one tensor must not meet loads or stores of another: the chunks run in no order.
+struct Span {
+  uint64_t begin, end;
+  int64_t index;
+};
+int check_apart(const void* const* src, void* const* dst, const int64_t* n, const int32_t* dtype, int64_t count) {
+  Span* spans = new (std::nothrow) Span[static_cast<size_t>(count) + 1];
+  if (!spans) return fail(TBE_ERR_INVALID_ARGUMENT, "tbe_grad_clip: out of host memory");
+  int64_t m = 0;
+  for (int64_t i = 0; i < count; ++i)
+    if (n[i] > 0) {
+      const uint64_t b = addr_bits(dst[i]);
+      spans[m++] = {b, b + static_cast<uint64_t>(n[i]) * any_elem_size(dtype[i]), i};
+    }
+  std::sort(spans, spans + m, [](const Span& x, const Span& y) { return x.begin < y.begin; });
+  int64_t bad = -1;
+  for (int64_t j = 1; j < m && bad < 0; ++j)
+    if (spans[j].begin < spans[j - 1].end) bad = spans[j].index;
+  for (int64_t i = 0; i < count && bad < 0; ++i) {
+    if (n[i] == 0 || src[i] == dst[i]) continue;  // in place: the stores above are its loads
+    const uint64_t b = addr_bits(src[i]), e = b + static_cast<uint64_t>(n[i]) * any_elem_size(dtype[i]);
+    const Span* s = std::lower_bound(spans, spans + m, b, [](const Span& x, uint64_t v) { return x.end <= v; });
+    if (s != spans + m && s->begin < e) bad = i;
+  }
+  delete[] spans;
+  if (bad >= 0)
+    return fail(TBE_ERR_INVALID_ARGUMENT, "tbe_grad_clip: tensor %lld shares memory with another one that is written",
+                static_cast<long long>(bad));
+  return TBE_OK;
+}
+
+template <int CAP>
+int norm_launches(const void* const* src, const int64_t* n, const int32_t* dtype, int count, double* partial, int* parts,
+                  cudaStream_t stream) {
+  static_assert(sizeof(Table<CAP>) + 64 <= 32764, "the table does not fit into a kernel's parameters");
+  *parts = 0;
+  Table<CAP> t;
+  int from = 0;
+  do {
+    const int to = count - from < CAP ? count : from + CAP;
+    TBE_REQUIRE(fill(t, src, nullptr, n, dtype, from, to), "tbe_grad_norm: too many elements");
+    const int grid = launch_grid(t.chunks);
+    {
+      KernelTimer timer("grad_norm_kernel", stream);
+      grad_norm_kernel<CAP><<<grid, kClipThreads, 0, stream>>>(t, partial + *parts);
+    }
+    TBE_CHECK_LAUNCH("grad_norm_kernel");
+    *parts += grid;
+    from = to;
+  } while (from < count);
+  return TBE_OK;
+}
+
+template <int CAP>
+int scale_launches(const void* const* src, void* const* dst, const int64_t* n, const int32_t* dtype, int count,
+                   const double* partial, int parts, double max_norm, double eps, bool in_place, float* norm,
+                   cudaStream_t stream) {
+  Table<CAP> t;
+  // backwards over the launches too
+  int to = count;
+  do {
+    const int from = to > CAP ? (to - 1) / CAP * CAP : 0;
+    TBE_REQUIRE(fill(t, src, dst, n, dtype, from, to), "tbe_grad_clip: too many elements");
+    {
+      KernelTimer timer("grad_scale_kernel", stream);
+      grad_scale_kernel<CAP><<<launch_grid(t.chunks), kClipThreads, 0, stream>>>(t, partial, parts, max_norm, eps, in_place,
+                                                                                 norm);
+    }
+    TBE_CHECK_LAUNCH("grad_scale_kernel");
+    norm = nullptr;
+    to = from;
+  } while (to > 0);
+  return TBE_OK;
+}
+
+int64_t launches_of(int64_t count) { return count <= kLargeTable ? 1 : (count + kLargeTable - 1) / kLargeTable; }
+
+}  // namespace
+}  // namespace tbe
+
+extern "C" int64_t tbe_grad_norm_workspace_bytes(int64_t count) {
+  using namespace tbe;
+  if (count < 0 || count >= (1ll << 24))
+    return fail(TBE_ERR_INVALID_ARGUMENT, "tbe_grad_norm_workspace_bytes: the number of tensors must be 0..2^24-1");
+  return launches_of(count) * device_sm_count() * kClipBlocksPerSM * static_cast<int64_t>(sizeof(double));
+}
+
+namespace tbe {
+namespace {
+int run_norm(const char* who, const void* const* src, const int64_t* n, const int32_t* dtype, int64_t count, void* workspace,
+             int64_t workspace_bytes, int* parts, cudaStream_t stream) {
+  if (const int rc = check_list(who, src, n, dtype, count)) return rc;
+  const int64_t need = tbe_grad_norm_workspace_bytes(count);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(TBE_ERR_WORKSPACE_TOO_SMALL, "%s: workspace of %lld bytes, %lld needed", who,
+                static_cast<long long>(workspace_bytes), static_cast<long long>(need));
+  TBE_REQUIRE(addr_bits(workspace) % 8 == 0, "%s: the workspace must be 8-byte aligned", who);
+  double* partial = static_cast<double*>(workspace);
+  return count <= kSmallTable ? norm_launches<kSmallTable>(src, n, dtype, static_cast<int>(count), partial, parts, stream)
+                              : norm_launches<kLargeTable>(src, n, dtype, static_cast<int>(count), partial, parts, stream);
+}
+}  // namespace
+}  // namespace tbe
+
+extern "C" int tbe_grad_norm(const void* const* tensors, const int64_t* numels, const int32_t* dtypes, int64_t count,
+                             float* norm, void* workspace, int64_t workspace_bytes, void* stream_v) {
+  using namespace tbe;
+  TBE_REQUIRE(norm, "tbe_grad_norm: null pointer argument");
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  int parts = 0;
+  if (const int rc = run_norm("tbe_grad_norm", tensors, numels, dtypes, count, workspace, workspace_bytes, &parts, stream))
+    return rc;
+  {
+    KernelTimer timer("grad_norm_finish_kernel", stream);
+    grad_norm_finish_kernel<<<1, kClipThreads, 0, stream>>>(static_cast<const double*>(workspace), parts, norm);
+  }
+  TBE_CHECK_LAUNCH("grad_norm_finish_kernel");
+  return TBE_OK;
+}
+
+extern "C" int tbe_grad_clip(const void* const* tensors, void* const* outputs, const int64_t* numels, const int32_t* dtypes,
+                             int64_t count, double max_norm, double eps, float* norm, void* workspace,
+                             int64_t workspace_bytes, void* stream_v) {
+  using namespace tbe;
+  TBE_REQUIRE(norm && (count == 0 || outputs), "tbe_grad_clip: null pointer argument");
+  TBE_REQUIRE(max_norm >= 0.0 && eps >= 0.0, "tbe_grad_clip: max_norm and eps must not be negative");
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  if (const int rc = check_list("tbe_grad_clip", tensors, numels, dtypes, count)) return rc;
+  bool in_place = true;
+  for (int64_t i = 0; i < count; ++i) {
+    if (numels[i] == 0) continue;
+    TBE_REQUIRE(outputs[i] && addr_bits(outputs[i]) % any_elem_size(dtypes[i]) == 0,
+                "tbe_grad_clip: output %lld is null or not aligned to its elements", static_cast<long long>(i));
+    in_place &= outputs[i] == tensors[i];
+  }
+  if (const int rc = check_apart(tensors, outputs, numels, dtypes, count)) return rc;
+  int parts = 0;
+  if (const int rc = run_norm("tbe_grad_clip", tensors, numels, dtypes, count, workspace, workspace_bytes, &parts, stream))
+    return rc;
+  const double* partial = static_cast<const double*>(workspace);
+  return count <= kSmallTable ? scale_launches<kSmallTable>(tensors, outputs, numels, dtypes, static_cast<int>(count), partial,
+                                                            parts, max_norm, eps, in_place, norm, stream)
+                              : scale_launches<kLargeTable>(tensors, outputs, numels, dtypes, static_cast<int>(count), partial,
+                                                            parts, max_norm, eps, in_place, norm, stream);
+}

@@ -6,6 +6,7 @@
 Differences, all opt-in or fixes:
   * ``pooling_mode="sum"|"mean"`` keyword (the reference only sums);
   * ``plan_ahead`` keyword: sort the lookups for the backward on a side stream while the forward runs;
+  * ``max_grad_norm`` keyword: the pooled gradient is scaled down to this 2-norm before the optimizer;
   * SGD sums the gradients of repeated rows before the update (the reference's kernel races on
     them, and its Python branch raises a TypeError at table_batched_embeddings_ops.py:66);
   * tensors must be on a CUDA device: there is no CPU path.
@@ -17,7 +18,7 @@ import numpy as np
 import torch
 from torch import nn
 
-from . import table_batched_embeddings
+from . import gradient_clipping, table_batched_embeddings
 
 
 class Optimizer(enum.Enum):
@@ -44,15 +45,26 @@ def _empty_sparse_grad(weights):
     return torch.empty(tuple(weights.shape), layout=torch.sparse_coo, dtype=weights.dtype, device=weights.device)
 
 
+def _limited(grad, max_norm):
+    """``grad`` scaled down to a 2-norm of at most ``max_norm``: a new tensor, since autograd may hand the
+    same gradient to others."""
+    if not gradient_clipping._dense(grad):
+        grad = grad.contiguous()
+    out = torch.empty_like(grad)
+    gradient_clipping.clip_grad_norm(grad, max_norm, out=out)
+    return out
+
+
 class LookupFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weights, table_offsets, indices, offsets, per_sample_weights, optimizer, optimizer_state,
-                learning_rate, eps, stochastic_rounding, pooling_mode="sum", plan_ahead=False):
+                learning_rate, eps, stochastic_rounding, pooling_mode="sum", plan_ahead=False, max_grad_norm=None):
         ctx.optimizer = optimizer
         ctx.learning_rate = learning_rate
         ctx.eps = eps
         ctx.stochastic_rounding = stochastic_rounding
         ctx.pooling_mode = pooling_mode
+        ctx.max_grad_norm = max_grad_norm
         ctx.plan = None
         ctx.save_for_backward(weights, table_offsets, indices, offsets, per_sample_weights, optimizer_state)
         if (plan_ahead and weights.requires_grad and optimizer != Optimizer.APPROX_ROWWISE_ADAGRAD):
@@ -67,6 +79,8 @@ class LookupFunction(torch.autograd.Function):
         weights, table_offsets, indices, offsets, per_sample_weights, optimizer_state = ctx.saved_tensors
         assert ctx.optimizer in (Optimizer.SGD, Optimizer.APPROX_ROWWISE_ADAGRAD, Optimizer.EXACT_ROWWISE_ADAGRAD)
         grad_per_sample_weight = None
+        if ctx.max_grad_norm is not None:
+            grad_output = _limited(grad_output, ctx.max_grad_norm)
         if ctx.optimizer == Optimizer.SGD:
             assert per_sample_weights is None
             table_batched_embeddings.backward_sgd(
@@ -83,7 +97,7 @@ class LookupFunction(torch.autograd.Function):
                 ctx.learning_rate, ctx.eps, ctx.stochastic_rounding, 1, pooling_mode=ctx.pooling_mode, plan=ctx.plan)
         ctx.plan = None
         return (_empty_sparse_grad(weights), None, None, None, grad_per_sample_weight, None, None, None, None,
-                None, None, None)
+                None, None, None, None)
 
 
 class TableBatchedEmbeddingBags(nn.Module):
@@ -91,12 +105,16 @@ class TableBatchedEmbeddingBags(nn.Module):
 
     ``forward(indices, offsets[, per_sample_weights])`` takes int32 ``indices`` flattened as
     ``[T][B][L]`` and int32 ``offsets`` of length ``T*B+1`` and returns ``[B, T, D]``.
+
+    ``max_grad_norm`` (None: no limit) scales the gradient of the returned ``[B, T, D]`` down to this 2-norm
+    before the fused optimizer uses it; the gradient of ``per_sample_weights`` is taken from the scaled one.
     """
 
     def __init__(self, num_tables, num_embeddings, embedding_dim, optimizer=Optimizer.SGD, learning_rate=0.01,
                  eps=None, stochastic_rounding=False, fp16=False, managed=EmbeddingLocation.DEVICE, *,
-                 pooling_mode="sum", plan_ahead=False):
+                 pooling_mode="sum", plan_ahead=False, max_grad_norm=None):
         super().__init__()
+        assert max_grad_norm is None or max_grad_norm >= 0
         assert managed in (EmbeddingLocation.DEVICE, EmbeddingLocation.HOST_MAPPED)
         assert pooling_mode in ("sum", "mean")
         dtype = torch.float16 if fp16 else torch.float32
@@ -121,12 +139,13 @@ class TableBatchedEmbeddingBags(nn.Module):
         self.stochastic_rounding = stochastic_rounding
         self.pooling_mode = pooling_mode
         self.plan_ahead = plan_ahead
+        self.max_grad_norm = max_grad_norm
 
     def forward(self, sharded_sparse_features, sharded_offsets, per_sample_weights=None):
         return LookupFunction.apply(
             self.embedding_weights, self.table_offsets, sharded_sparse_features, sharded_offsets,
             per_sample_weights, self.optimizer, self.optimizer_state, self.learning_rate, self.eps,
-            self.stochastic_rounding, self.pooling_mode, self.plan_ahead)
+            self.stochastic_rounding, self.pooling_mode, self.plan_ahead, self.max_grad_norm)
 
 
 class MixedDimLookupFunction(torch.autograd.Function):
