@@ -112,6 +112,23 @@ def lib():
     return _lib
 
 
+_glue = None
+
+
+def glue():
+    """The compiled PyTorch side of expert routing and gradient clipping, loaded on first use."""
+    global _glue
+    if _glue is None:
+        lib()
+        try:
+            from . import _torch_glue
+        except ImportError as e:
+            raise RuntimeError("_torch_glue.so is not built or does not fit this PyTorch (%s). Build it with "
+                               "`python -m sparse_ads_baselines_b200.build`; there is no Python fallback." % e) from e
+        _glue = _torch_glue
+    return _glue
+
+
 def last_error():
     return lib().tbe_last_error_string().decode("utf-8", "replace")
 

@@ -3,18 +3,22 @@
 Run as ``python -m sparse_ads_baselines_b200.build`` or call :func:`build`.  Each ``csrc/*.cu`` is
 compiled to an object file (in parallel, skipped when up to date) and linked into
 ``sparse_ads_baselines_b200/libtbe_b200.so``; the CUDA runtime is linked statically so the library
-depends on nothing but the driver.
+depends on nothing but the driver.  ``csrc/torch_glue.cpp`` -- the PyTorch side of expert routing and
+gradient clipping -- becomes the extension module ``_torch_glue.so`` beside it, linked to that library and
+to the PyTorch that builds it.
 """
 import concurrent.futures
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libtbe_b200.so")
+GLUE = os.path.join(HERE, "_torch_glue.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -37,6 +41,26 @@ def _newer(target, deps):
         return False
     t = os.path.getmtime(target)
     return all(os.path.getmtime(d) <= t for d in deps)
+
+
+def _build_glue(force):
+    import torch
+    from torch.utils import cpp_extension
+    src = os.path.join(CSRC, "torch_glue.cpp")
+    header = os.path.join(HERE, "..", "include", "tbe_b200.h")
+    if not force and _newer(GLUE, [src, header, os.path.abspath(__file__), torch.__file__]):
+        return
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    includes = cpp_extension.include_paths() + [os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    cmd = (["g++", "-shared", "-fPIC", "-O2", "-std=c++17", "-fvisibility=hidden", "-w",
+            "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, src, "-o", GLUE]
+           + [f for p in includes for f in ("-isystem", p)]
+           + [f for p in cpp_extension.library_paths() for f in ("-L" + p,)]
+           + ["-L" + HERE, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN",
+              "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10"])
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("g++ failed for torch_glue.cpp:\n%s\n%s" % (r.stdout, r.stderr))
 
 
 def build(verbose=False, force=False, ptxas_info=False):
@@ -71,6 +95,7 @@ def build(verbose=False, force=False, ptxas_info=False):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("link failed:\n%s\n%s" % (r.stdout, r.stderr))
+    _build_glue(force)
     return LIB
 
 
