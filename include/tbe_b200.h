@@ -72,7 +72,8 @@ TBE_API int64_t tbe_library_launch_count(void);
  *   sort_bucket                                  wanted mean bucket size of the table-segmented sort
  *   split_runs                                   1: one CTA per queued long run, never several
  *   bwd_stride                                   backward apply hands out its tiles 1: with a fixed stride, 2: by a ticket
- *                                                counter (default: tickets once the pooled gradient exceeds a third of L2) */
+ *                                                counter (default: tickets once the pooled gradient exceeds a third of L2)
+ *   row_threads                                  most threads per launch of tbe_expert_dispatch / _combine */
 TBE_API int tbe_set_tuning(const char* name, int value);
 
 /* Per-launch timing for benchmarks: while enabled, every kernel launch of this library
@@ -321,7 +322,7 @@ TBE_API int tbe_expert_gate_backward(const void* grad_weights, const void* logit
 /* Stable sort of M choices (experts[M] = [N][k] flattened) by expert: positions[i] is the row choice i
  * takes, order[positions[i]] = i, and rows offsets[e] .. offsets[e+1) (int32 [E+1]) are expert e's.  Ids
  * outside 0..E-1 -- unassigned slots, experts of another rank -- sort behind all experts, at rows
- * offsets[E] .. M-1.  One kernel for up to 8192 choices, two above (workspace:
+ * offsets[E] .. M-1.  One kernel for up to 131072 choices, two above (workspace:
  * tbe_expert_plan_workspace_bytes, 0 for one kernel; it needs no initialisation). */
 TBE_API int64_t tbe_expert_plan_workspace_bytes(int64_t M, int64_t E);
 TBE_API int tbe_expert_plan(const int32_t* experts, int32_t* offsets, int32_t* positions, int32_t* order, int64_t M,

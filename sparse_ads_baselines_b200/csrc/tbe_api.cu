@@ -21,7 +21,8 @@ std::atomic<int64_t> g_library_launches{0};
 std::atomic<int> g_tuning[kTuneCount];
 const char* const kTuningNames[kTuneCount] = {"fwd_unroll", "fwd_threads", "bwd_threads", "bwd_unroll",
                                               "long_segment", "fwd_blocks_per_sm", "bwd_blocks_per_sm", "bwd_vpl",
-                                              "bwd_sort", "sort_bucket", "split_runs", "bwd_stride"};
+                                              "bwd_sort", "sort_bucket", "split_runs", "bwd_stride",
+                                              "row_threads"};
 }  // namespace
 
 namespace {

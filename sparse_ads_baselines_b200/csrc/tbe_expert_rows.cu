@@ -13,13 +13,23 @@
 // (or k rows are read and one stored), so the traffic is the algorithm's, no sum needs an atomic and the
 // results do not depend on the order of anything.  All of it is bound by HBM.  A position outside the
 // rows is skipped by every kernel, so a wrong plan cannot reach memory outside the tensors.
+#include <cooperative_groups.h>
+
 #include "tbe_elem.cuh"
 
 namespace tbe {
 namespace {
 
 constexpr int kMaxExperts = 1024;
-constexpr int kPlanSlice = 8192;  // choices per CTA of the two-kernel plan, at least
+namespace cg = cooperative_groups;
+
+// How many CTAs sort a plan, by its number of choices: one, one cluster (totals exchanged through
+// distributed shared memory), or a grid with a counting kernel in front (totals through global memory).
+constexpr int kPlanOne = 4096;
+constexpr int kPlanCluster = 8;
+constexpr int kPlanClusterMost = 131072;
+constexpr int kPlanSlice = 8192;  // choices per CTA of the grid, at least
+enum PlanMode { kOne, kCluster, kGrid };
 
 // ---------------------------------------------------------------- plan
 struct PlanArgs {
@@ -59,15 +69,16 @@ __device__ void block_exclusive_scan(int32_t* v, int n, int32_t* warp_sums) {
 // One CTA sorts its slice: every warp counts a contiguous part per bin, the parts are prefix-summed warp
 // by warp, and a second pass in the same order places each choice behind the earlier ones of its bin.
 // The order is therefore the stable one, whatever the atomics of the counting did.
-//   shared: hist[warps][E+1], start[E+1], before[E+1], 32 words
-template <bool MULTI>
+//   shared: hist[warps][E+1], start[E+1], before[E+1], own[E+1], 32 words
+template <int MODE>
 __global__ void __launch_bounds__(1024) plan_place_kernel(PlanArgs a) {
   extern __shared__ int32_t plan_smem[];
   const int E1 = a.E + 1, warps = blockDim.x >> 5, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int32_t* hist = plan_smem;
-  int32_t* start = hist + warps * E1;
-  int32_t* before = start + E1;
-  int32_t* warp_sums = before + E1;
+  int32_t* start = hist + warps * E1;  // where a bin begins
+  int32_t* before = start + E1;        // choices of the bin in the CTAs in front of this one
+  int32_t* own = before + E1;          // choices of the bin in this CTA
+  int32_t* warp_sums = own + E1;
   const int64_t s0 = static_cast<int64_t>(blockIdx.x) * a.slice;
   const int begin = static_cast<int>(s0 < a.M ? s0 : a.M), len = min(a.slice, a.M - begin);
   const int part = ((len + warps - 1) / warps + 31) & ~31;
@@ -76,7 +87,7 @@ __global__ void __launch_bounds__(1024) plan_place_kernel(PlanArgs a) {
   for (int i = threadIdx.x; i < warps * E1 + 2 * E1; i += blockDim.x) hist[i] = 0;
   __syncthreads();
   for (int i = wb + lane; i < we; i += 32) atomicAdd(&hist[warp * E1 + bin_of(__ldg(a.experts + i), a.E)], 1);
-  if (MULTI) {  // totals of every bin, and what the CTAs in front of this one put there
+  if (MODE == kGrid) {
     const int n = gridDim.x * E1, mine = blockIdx.x * E1;
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
       const int32_t c = __ldg(a.counts + i);
@@ -89,18 +100,42 @@ __global__ void __launch_bounds__(1024) plan_place_kernel(PlanArgs a) {
   }
   __syncthreads();
   for (int b = threadIdx.x; b < E1; b += blockDim.x) {
-    int32_t run = MULTI ? before[b] : 0;
+    int32_t run = 0;
     for (int w = 0; w < warps; ++w) {
       const int32_t c = hist[w * E1 + b];
       hist[w * E1 + b] = run;
       run += c;
     }
-    if (!MULTI) start[b] = run;
+    if (MODE == kOne) start[b] = run;
+    if (MODE == kCluster) own[b] = run;
   }
-  __syncthreads();
+  if (MODE == kCluster) {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();  // every CTA's own totals are in place
+    const int rank = static_cast<int>(cluster.block_rank());
+    for (int b = threadIdx.x; b < E1; b += blockDim.x) {
+      int32_t total = 0, front = 0;
+#pragma unroll
+      for (int c = 0; c < kPlanCluster; ++c) {
+        const int32_t t = cluster.map_shared_rank(own, c)[b];
+        total += t;
+        if (c < rank) front += t;
+      }
+      start[b] = total;
+      before[b] = front;
+    }
+    cluster.sync();  // nobody's totals are read any more
+  } else {
+    __syncthreads();
+  }
   block_exclusive_scan(start, E1, warp_sums);
   if (blockIdx.x == 0)
     for (int b = threadIdx.x; b < E1; b += blockDim.x) a.offsets[b] = start[b];
+  if (MODE != kOne) {
+    __syncthreads();
+    for (int b = threadIdx.x; b < E1; b += blockDim.x) start[b] += before[b];
+    __syncthreads();
+  }
 
   int32_t* next = hist + warp * E1;
   for (int i0 = wb; i0 < we; i0 += 32) {
@@ -134,13 +169,15 @@ __global__ void __launch_bounds__(1024) plan_count_kernel(PlanArgs a) {
 }
 
 struct PlanShape {
+  PlanMode mode;
   int ctas, slice;
 };
 PlanShape plan_shape(int64_t M) {
+  if (M <= kPlanOne) return {kOne, 1, static_cast<int>(M)};
+  if (M <= kPlanClusterMost) return {kCluster, kPlanCluster, static_cast<int>((M + kPlanCluster - 1) / kPlanCluster)};
   int64_t ctas = (M + kPlanSlice - 1) / kPlanSlice;
   if (ctas > 148) ctas = 148;
-  if (ctas < 1) ctas = 1;
-  return {static_cast<int>(ctas), static_cast<int>((M + ctas - 1) / ctas)};
+  return {kGrid, static_cast<int>(ctas), static_cast<int>((M + ctas - 1) / ctas)};
 }
 
 // ---------------------------------------------------------------- rows
@@ -154,8 +191,8 @@ struct RowArgs {
   int64_t row_bytes;  // stride of position-ordered and freshly written rows
   int32_t M;
   int k;
-  uint32_t nvec, items;  // vectors per row, (sample, vector) pairs of this launch
-  FastDiv div;           // by nvec
+  uint32_t nvec, per_row, items;  // vectors per row, threads per row, threads of this launch
+  FastDiv div;                    // by per_row
 };
 
 __device__ __forceinline__ uint32_t kept_rows(const int32_t* kept, int32_t M) {
@@ -163,46 +200,51 @@ __device__ __forceinline__ uint32_t kept_rows(const int32_t* kept, int32_t M) {
   return static_cast<uint32_t>(n < 0 ? 0 : n > M ? M : n);
 }
 
-// A thread takes U (sample, vector) pairs a CTA width apart: U independent loads, then k stores each.
+// A thread takes U vectors of one sample's row, a U-th of the row apart, so that a warp's loads stay
+// contiguous and the positions are looked up once for all of them: U independent loads, then k stores each.
 template <int VB, int U>
 __global__ void __launch_bounds__(256) dispatch_kernel(RowArgs a) {
-  const uint32_t base = blockIdx.x * (256u * U) + threadIdx.x;
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+  if (i >= a.items) return;
+  const uint32_t t = fastdiv(i, a.div), v0 = i - t * a.per_row;
+  const char* src = a.x + t * a.x_stride;
   Raw<VB> r[U];
-  uint32_t t[U], v[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const uint32_t i = base + u * 256u;
-    t[u] = fastdiv(i, a.div);
-    v[u] = (i - t[u] * a.nvec) * VB;
-    if (i < a.items) r[u] = ld_stream<VB>(a.x + t[u] * a.x_stride + v[u]);
+    const uint32_t v = v0 + u * a.per_row;
+    if (v < a.nvec) r[u] = ld_stream<VB>(src + static_cast<int64_t>(v) * VB);
   }
   const uint32_t kept = kept_rows(a.kept, a.M), M = static_cast<uint32_t>(a.M);
+  const int32_t* pos = a.positions + static_cast<int64_t>(t) * a.k;
+  for (int s = 0; s < a.k; ++s) {
+    const uint32_t p = static_cast<uint32_t>(__ldg(pos + s));
+    if (p >= M) continue;
+    char* dst = a.out + p * a.row_bytes;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if (base + u * 256u >= a.items) break;
-    const int32_t* pos = a.positions + static_cast<int64_t>(t[u]) * a.k;
-    for (int s = 0; s < a.k; ++s) {
-      const uint32_t p = static_cast<uint32_t>(__ldg(pos + s));
-      if (p < M) st_row<VB>(a.out + p * a.row_bytes + v[u], p < kept ? r[u] : raw_none<VB>());
+    for (int u = 0; u < U; ++u) {
+      const uint32_t v = v0 + u * a.per_row;
+      if (v < a.nvec) st_row<VB>(dst + static_cast<int64_t>(v) * VB, p < kept ? r[u] : raw_none<VB>());
     }
   }
 }
 
-// A thread sums one vector of a sample's row; KB row loads are in flight together.
-template <typename T, int VB, int KB>
-__global__ void __launch_bounds__(256) combine_kernel(RowArgs a) {
+// The same U vectors, summed over the sample's rows; KB * U row loads are in flight together.
+template <typename T, int VB, int U, int KB>
+__global__ void __launch_bounds__(256, 4) combine_kernel(RowArgs a) {
   using A = typename Acc<T>::type;
   constexpr int NE = VB / sizeof(T);
   const uint32_t i = blockIdx.x * 256u + threadIdx.x;
   if (i >= a.items) return;
-  const uint32_t t = fastdiv(i, a.div), v = (i - t * a.nvec) * VB;
+  const uint32_t t = fastdiv(i, a.div), v0 = i - t * a.per_row;
   const int64_t at = static_cast<int64_t>(t) * a.k;
   const uint32_t kept = kept_rows(a.kept, a.M);
-  A acc[NE];
+  A acc[U][NE];
 #pragma unroll
-  for (int e = 0; e < NE; ++e) acc[e] = A(0);
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int e = 0; e < NE; ++e) acc[u][e] = A(0);
   for (int s0 = 0; s0 < a.k; s0 += KB) {
-    Raw<VB> r[KB];
+    Raw<VB> r[KB][U];
     bool in[KB];
     A w[KB];
 #pragma unroll
@@ -211,18 +253,31 @@ __global__ void __launch_bounds__(256) combine_kernel(RowArgs a) {
       const uint32_t p = on ? static_cast<uint32_t>(__ldg(a.positions + at + s0 + s)) : 0xffffffffu;
       in[s] = p < kept;
       w[s] = in[s] && a.weights ? __ldg(static_cast<const A*>(a.weights) + at + s0 + s) : A(1);
-      if (in[s]) r[s] = ld_stream<VB>(a.x + p * a.x_stride + v);
+      const char* src = a.x + p * a.x_stride;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t v = v0 + u * a.per_row;
+        if (in[s] && v < a.nvec) r[s][u] = ld_stream<VB>(src + static_cast<int64_t>(v) * VB);
+      }
     }
 #pragma unroll
     for (int s = 0; s < KB; ++s) {
       if (!in[s]) continue;
-      A e[NE];
-      expand<T, VB>(r[s], e);
 #pragma unroll
-      for (int j = 0; j < NE; ++j) acc[j] += w[s] * e[j];
+      for (int u = 0; u < U; ++u) {
+        A e[NE];
+        expand<T, VB>(r[s][u], e);
+#pragma unroll
+        for (int j = 0; j < NE; ++j) acc[u][j] += w[s] * e[j];
+      }
     }
   }
-  st_row<VB>(a.out + t * a.row_bytes + v, narrow<T, VB>(acc));
+  char* dst = a.out + t * a.row_bytes;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t v = v0 + u * a.per_row;
+    if (v < a.nvec) st_row<VB>(dst + static_cast<int64_t>(v) * VB, narrow<T, VB>(acc[u]));
+  }
 }
 
 struct GradArgs {
@@ -241,9 +296,9 @@ struct GradArgs {
   int nvec;
 };
 
-// G lanes per sample walk its row: the upstream row is held in registers while KB expert rows are read
-// against it (dot products) and KB scaled copies are stored.
-template <typename T, int VB, int G, int KB>
+// G lanes per sample walk its row, U vectors at a time: the upstream row is held in registers while KB
+// expert rows are read against it (dot products) and KB scaled copies are stored.
+template <typename T, int VB, int U, int G, int KB>
 __global__ void __launch_bounds__(G == 128 ? 128 : 256) combine_backward_kernel(GradArgs a) {
   using A = typename Acc<T>::type;
   constexpr int NE = VB / sizeof(T), kThreads = G == 128 ? 128 : 256;
@@ -263,30 +318,38 @@ __global__ void __launch_bounds__(G == 128 ? 128 : 256) combine_backward_kernel(
       w[s] = on ? __ldg(static_cast<const A*>(a.weights) + t * a.k + s0 + s) : A(0);
       dot[s] = A(0);
     }
-    for (int v = live ? sub : a.nvec; v < a.nvec; v += G) {
-      const int64_t off = static_cast<int64_t>(v) * VB;
-      const Raw<VB> gr = ld_stream<VB>(go + off);
-      Raw<VB> r[KB];
+    for (int v0 = live ? sub : a.nvec; v0 < a.nvec; v0 += G * U) {
+      Raw<VB> gr[U], r[KB][U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) gr[u] = v0 + u * G < a.nvec ? ld_stream<VB>(go + static_cast<int64_t>(v0 + u * G) * VB) : raw_none<VB>();
       if (a.grad_weights) {
 #pragma unroll
         for (int s = 0; s < KB; ++s)
-          if (p[s] < kept) r[s] = ld_stream<VB>(a.y + p[s] * a.row_bytes + off);
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (p[s] < kept && v0 + u * G < a.nvec)
+              r[s][u] = ld_stream<VB>(a.y + p[s] * a.row_bytes + static_cast<int64_t>(v0 + u * G) * VB);
       }
-      A g[NE];
-      expand<T, VB>(gr, g);
 #pragma unroll
-      for (int s = 0; s < KB; ++s) {
-        if (a.grad_weights && p[s] < kept) {
-          A e[NE];
-          expand<T, VB>(r[s], e);
+      for (int u = 0; u < U; ++u) {
+        if (v0 + u * G >= a.nvec) break;
+        const int64_t off = static_cast<int64_t>(v0 + u * G) * VB;
+        A g[NE];
+        expand<T, VB>(gr[u], g);
 #pragma unroll
-          for (int j = 0; j < NE; ++j) dot[s] += g[j] * e[j];
-        }
-        if (a.grad_y && p[s] < M) {
-          A d[NE];
+        for (int s = 0; s < KB; ++s) {
+          if (a.grad_weights && p[s] < kept) {
+            A e[NE];
+            expand<T, VB>(r[s][u], e);
 #pragma unroll
-          for (int j = 0; j < NE; ++j) d[j] = p[s] < kept ? w[s] * g[j] : A(0);
-          st_row<VB>(a.grad_y + p[s] * a.row_bytes + off, narrow<T, VB>(d));
+            for (int j = 0; j < NE; ++j) dot[s] += g[j] * e[j];
+          }
+          if (a.grad_y && p[s] < M) {
+            A d[NE];
+#pragma unroll
+            for (int j = 0; j < NE; ++j) d[j] = p[s] < kept ? w[s] * g[j] : A(0);
+            st_row<VB>(a.grad_y + p[s] * a.row_bytes + off, narrow<T, VB>(d));
+          }
         }
       }
     }
@@ -315,55 +378,51 @@ __global__ void __launch_bounds__(G == 128 ? 128 : 256) combine_backward_kernel(
 }
 
 // ---------------------------------------------------------------- launches
-// 32-bit pair indices: a launch covers as many samples as fit below 2^32 pairs.
-int64_t rows_per_launch(int64_t nvec) {
-  const int64_t n = (0xffffffffll - 4096) / nvec;
-  return n < 1 ? 1 : n;
+// Vectors per thread: 16 bytes' worth, so that narrow vectors have as many loads in flight as wide ones.
+// (5003 rows of 1001 fp32 values, six choices each: one 4-byte vector a thread moved 3.6 and 3.0 TB/s.)
+constexpr int vectors_per_thread(int vb) { return vb == 16 ? 1 : vb == 8 ? 2 : 4; }
+
+// 32-bit thread indices: a launch covers as many samples as fit below 2^32 threads.  body(first sample,
+// arguments of the launch, blocks) launches one.
+template <typename F>
+int per_sample_launches(const char* name, RowArgs a, int64_t N, int vb, int u, cudaStream_t stream, F body) {
+  a.nvec = static_cast<uint32_t>(a.row_bytes / vb);
+  a.per_row = (a.nvec + u - 1) / u;
+  a.div = make_fastdiv(a.per_row);
+  const int64_t knob = tuning(kTuneRowThreads), most = knob > 0 ? knob : 0xffffffffll - 4096;
+  const int64_t step = most > a.per_row ? most / a.per_row : 1;  // per_row <= 2^28
+  for (int64_t n0 = 0; n0 < N; n0 += step) {
+    const int64_t n = N - n0 < step ? N - n0 : step;
+    RowArgs b = a;
+    b.positions = a.positions + n0 * a.k;
+    b.items = static_cast<uint32_t>(n * a.per_row);
+    {
+      KernelTimer timer(name, stream);
+      body(n0, b, static_cast<unsigned>((static_cast<int64_t>(b.items) + 255) / 256));
+    }
+    TBE_CHECK_LAUNCH(name);
+  }
+  return TBE_OK;
 }
 
 template <int VB>
-int launch_dispatch(RowArgs a, int64_t N, cudaStream_t stream) {
-  constexpr int U = 2;
-  a.nvec = static_cast<uint32_t>(a.row_bytes / VB);
-  a.div = make_fastdiv(a.nvec);
-  const int64_t step = rows_per_launch(a.nvec);
-  for (int64_t n0 = 0; n0 < N; n0 += step) {
-    RowArgs b = a;
-    const int64_t n = N - n0 < step ? N - n0 : step;
+int launch_dispatch(const RowArgs& a, int64_t N, cudaStream_t stream) {
+  constexpr int U = 2 * vectors_per_thread(VB);
+  return per_sample_launches("dispatch_kernel", a, N, VB, U, stream, [&](int64_t n0, RowArgs b, unsigned blocks) {
     b.x = a.x + n0 * a.x_stride;
-    b.positions = a.positions + n0 * a.k;
-    b.items = static_cast<uint32_t>(n * a.nvec);
-    const uint32_t blocks = static_cast<uint32_t>((static_cast<int64_t>(b.items) + 256 * U - 1) / (256 * U));
-    {
-      KernelTimer timer("dispatch_kernel", stream);
-      dispatch_kernel<VB, U><<<blocks, 256, 0, stream>>>(b);
-    }
-    TBE_CHECK_LAUNCH("dispatch_kernel");
-  }
-  return TBE_OK;
+    dispatch_kernel<VB, U><<<blocks, 256, 0, stream>>>(b);
+  });
 }
 
 template <typename T, int VB, int KB>
-int launch_combine_k(RowArgs a, int64_t N, cudaStream_t stream) {
+int launch_combine_k(const RowArgs& a, int64_t N, cudaStream_t stream) {
   using A = typename Acc<T>::type;
-  a.nvec = static_cast<uint32_t>(a.row_bytes / VB);
-  a.div = make_fastdiv(a.nvec);
-  const int64_t step = rows_per_launch(a.nvec);
-  for (int64_t n0 = 0; n0 < N; n0 += step) {
-    RowArgs b = a;
-    const int64_t n = N - n0 < step ? N - n0 : step;
-    b.positions = a.positions + n0 * a.k;
+  constexpr int U = vectors_per_thread(VB);
+  return per_sample_launches("combine_kernel", a, N, VB, U, stream, [&](int64_t n0, RowArgs b, unsigned blocks) {
     b.weights = a.weights ? static_cast<const A*>(a.weights) + n0 * a.k : nullptr;
     b.out = a.out + n0 * a.row_bytes;
-    b.items = static_cast<uint32_t>(n * a.nvec);
-    const uint32_t blocks = static_cast<uint32_t>((static_cast<int64_t>(b.items) + 255) / 256);
-    {
-      KernelTimer timer("combine_kernel", stream);
-      combine_kernel<T, VB, KB><<<blocks, 256, 0, stream>>>(b);
-    }
-    TBE_CHECK_LAUNCH("combine_kernel");
-  }
-  return TBE_OK;
+    combine_kernel<T, VB, U, KB><<<blocks, 256, 0, stream>>>(b);
+  });
 }
 
 template <typename T, int VB>
@@ -393,7 +452,7 @@ int launch_backward_gk(const GradArgs& a, cudaStream_t stream) {
   const int64_t blocks = (a.N + kThreads / G - 1) / (kThreads / G);
   {
     KernelTimer timer("combine_backward_kernel", stream);
-    combine_backward_kernel<T, VB, G, KB><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(a);
+    combine_backward_kernel<T, VB, vectors_per_thread(VB), G, KB><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(a);
   }
   TBE_CHECK_LAUNCH("combine_backward_kernel");
   return TBE_OK;
@@ -444,7 +503,7 @@ extern "C" int64_t tbe_expert_plan_workspace_bytes(int64_t M, int64_t E) {
   if (M < 0 || M >= (1ll << 31) || E < 1 || E > kMaxExperts)
     return fail(TBE_ERR_INVALID_ARGUMENT, "tbe_expert_plan_workspace_bytes: M must be 0..2^31-1 and E 1..%d", kMaxExperts);
   const PlanShape s = plan_shape(M);
-  return s.ctas == 1 ? 0 : static_cast<int64_t>(s.ctas) * (E + 1) * 4;
+  return s.mode == kGrid ? static_cast<int64_t>(s.ctas) * (E + 1) * 4 : 0;
 }
 
 extern "C" int tbe_expert_plan(const int32_t* experts, int32_t* offsets, int32_t* positions, int32_t* order, int64_t M,
@@ -461,11 +520,11 @@ extern "C" int tbe_expert_plan(const int32_t* experts, int32_t* offsets, int32_t
   PlanArgs a{experts, offsets, positions, order, static_cast<int32_t*>(workspace), static_cast<int32_t>(M),
              static_cast<int32_t>(E), s.slice};
   const int threads = M <= 1024 ? 256 : 1024;
-  const size_t shared = (static_cast<size_t>(threads / 32 + 2) * (E + 1) + 32) * 4;
-  auto place = s.ctas == 1 ? plan_place_kernel<false> : plan_place_kernel<true>;
+  const size_t shared = (static_cast<size_t>(threads / 32 + 3) * (E + 1) + 32) * 4;  // at most 144 KB
+  auto place = s.mode == kOne ? plan_place_kernel<kOne> : s.mode == kCluster ? plan_place_kernel<kCluster> : plan_place_kernel<kGrid>;
   if (shared > 48 * 1024)
     TBE_CUDA_TRY(cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)));
-  if (s.ctas > 1) {
+  if (s.mode == kGrid) {
     {
       KernelTimer timer("plan_count_kernel", stream);
       plan_count_kernel<<<s.ctas, 1024, (E + 1) * 4, stream>>>(a);
@@ -474,7 +533,22 @@ extern "C" int tbe_expert_plan(const int32_t* experts, int32_t* offsets, int32_t
   }
   {
     KernelTimer timer("plan_place_kernel", stream);
-    place<<<s.ctas, threads, shared, stream>>>(a);
+    if (s.mode == kCluster) {
+      cudaLaunchAttribute attr;
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = kPlanCluster;
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(kPlanCluster);
+      cfg.blockDim = dim3(static_cast<unsigned>(threads));
+      cfg.dynamicSmemBytes = shared;
+      cfg.stream = stream;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      TBE_CUDA_TRY(cudaLaunchKernelEx(&cfg, place, a));
+    } else {
+      place<<<s.ctas, threads, shared, stream>>>(a);
+    }
   }
   TBE_CHECK_LAUNCH("plan_place_kernel");
   return TBE_OK;

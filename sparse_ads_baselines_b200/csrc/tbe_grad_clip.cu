@@ -11,6 +11,8 @@
 // Bound by HBM.  The norm has to be known before the first element is scaled, so a list larger than L2 is
 // read twice; the scaling pass runs through the chunks backwards, so that what the norm pass read last is
 // still in L2.  In place and with c == 1 there is nothing to store and the second pass ends at once.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <new>
 
@@ -19,9 +21,14 @@
 namespace tbe {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kClipThreads = 256;
 constexpr int kClipBlocksPerSM = 8;
 constexpr int kChunk = 16384;      // elements
+constexpr int kSmallChunk = 1024;  // elements per warp of the one-kernel form
+constexpr int kSmallMost = 1 << 18;
+constexpr int kSmallCluster = 8;
 constexpr int kSmallTable = 64;    // tensors whose table fits a small parameter block
 constexpr int kLargeTable = 1024;  // and the largest (30 KB of parameters)
 
@@ -67,21 +74,22 @@ __device__ __forceinline__ double sum_squares(const Raw<VB>& r) {
   return d;
 }
 
+// By `threads` threads of which this one is `me`.
 template <typename T>
-__device__ double chunk_squares(const T* p, int n) {
+__device__ double chunk_squares(const T* p, int n, int me, int threads, uint64_t policy) {
   constexpr int NV = 16 / sizeof(T), U = 4;
   const int head = min(n, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / static_cast<int>(sizeof(T)));
   const int nvec = (n - head) / NV, tail = head + nvec * NV;
   double s = 0.0;
-  for (int i = threadIdx.x; i < head; i += kClipThreads) s += sum_squares<T, sizeof(T)>(ld_stream<sizeof(T)>(p + i));
-  for (int i = tail + threadIdx.x; i < n; i += kClipThreads) s += sum_squares<T, sizeof(T)>(ld_stream<sizeof(T)>(p + i));
+  for (int i = me; i < head; i += threads) s += sum_squares<T, sizeof(T)>(ld_stream<sizeof(T)>(p + i));
+  for (int i = tail + me; i < n; i += threads) s += sum_squares<T, sizeof(T)>(ld_stream<sizeof(T)>(p + i));
   const T* q = p + head;
-  for (int v = threadIdx.x; v < nvec; v += kClipThreads * U) {
+  for (int v = me; v < nvec; v += threads * U) {
     Raw<16> r[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = v + u * kClipThreads;
-      r[u] = i < nvec ? ld_stream<16>(q + static_cast<int64_t>(i) * NV) : raw_none<16>();
+      const int i = v + u * threads;
+      r[u] = i < nvec ? ld_stream_hint<16>(q + static_cast<int64_t>(i) * NV, policy) : raw_none<16>();
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) s += sum_squares<T, 16>(r[u]);
@@ -103,21 +111,40 @@ __device__ __forceinline__ double block_sum(double v) {
   return s;
 }
 
+// The elements of chunk c, in chunks of `chunk` elements: tensor, first element, number.
+struct Piece {
+  int tensor;
+  int64_t at;
+  int n;
+};
 template <int CAP>
-__global__ void __launch_bounds__(kClipThreads) grad_norm_kernel(const __grid_constant__ Table<CAP> t, double* partial) {
-  double s = 0.0;
-  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-    const int k = tensor_of(t, c);
-    const int64_t at = static_cast<int64_t>(c - t.first[k]) * kChunk;
-    const int64_t left = t.n[k] - at;
-    const int n = static_cast<int>(left < kChunk ? left : kChunk);
-    switch (t.dtype[k]) {
-      case TBE_F16: s += chunk_squares(static_cast<const __half*>(t.src[k]) + at, n); break;
-      case TBE_BF16: s += chunk_squares(static_cast<const __nv_bfloat16*>(t.src[k]) + at, n); break;
-      case TBE_F32: s += chunk_squares(static_cast<const float*>(t.src[k]) + at, n); break;
-      default: s += chunk_squares(static_cast<const double*>(t.src[k]) + at, n); break;
-    }
+__device__ __forceinline__ Piece piece_of(const Table<CAP>& t, int c, int chunk) {
+  Piece p;
+  p.tensor = tensor_of(t, c);
+  p.at = static_cast<int64_t>(c - t.first[p.tensor]) * chunk;
+  const int64_t left = t.n[p.tensor] - p.at;
+  p.n = static_cast<int>(left < chunk ? left : chunk);
+  return p;
+}
+
+template <int CAP>
+__device__ __forceinline__ double piece_squares(const Table<CAP>& t, const Piece& p, int me, int threads, uint64_t policy) {
+  const void* src = t.src[p.tensor];
+  switch (t.dtype[p.tensor]) {
+    case TBE_F16: return chunk_squares(static_cast<const __half*>(src) + p.at, p.n, me, threads, policy);
+    case TBE_BF16: return chunk_squares(static_cast<const __nv_bfloat16*>(src) + p.at, p.n, me, threads, policy);
+    case TBE_F32: return chunk_squares(static_cast<const float*>(src) + p.at, p.n, me, threads, policy);
+    default: return chunk_squares(static_cast<const double*>(src) + p.at, p.n, me, threads, policy);
   }
+}
+
+// Chunks from `keep` on stay in L2 for the scaling pass, which begins with them; the others pass through.
+template <int CAP>
+__global__ void __launch_bounds__(kClipThreads) grad_norm_kernel(const __grid_constant__ Table<CAP> t, double* partial, int keep) {
+  const uint64_t pass = l2_policy_evict_first(), stay = l2_policy_evict_normal();
+  double s = 0.0;
+  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x)
+    s += piece_squares(t, piece_of(t, c, kChunk), threadIdx.x, kClipThreads, c < keep ? pass : stay);
   s = block_sum(s);
   if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
@@ -133,10 +160,10 @@ __global__ void __launch_bounds__(kClipThreads) grad_norm_finish_kernel(const do
   if (threadIdx.x == 0) *norm = static_cast<float>(r);
 }
 
-template <typename T>
-__device__ void scale_chunk(const T* src, T* dst, int n, double c) {
+template <int U, typename T>
+__device__ void scale_chunk(const T* src, T* dst, int n, double c, int me, int threads, uint64_t policy) {
   using A = typename Acc<T>::type;
-  constexpr int NV = 16 / sizeof(T), U = 4;
+  constexpr int NV = 16 / sizeof(T);
   const A f = static_cast<A>(c);
   const uintptr_t s = reinterpret_cast<uintptr_t>(src), d = reinterpret_cast<uintptr_t>(dst);
   int head = min(n, static_cast<int>((16 - (s & 15)) & 15) / static_cast<int>(sizeof(T)));
@@ -146,57 +173,102 @@ __device__ void scale_chunk(const T* src, T* dst, int n, double c) {
     nvec = 0;
   }
   const int tail = head + nvec * NV;
-  for (int i = threadIdx.x; i < head; i += kClipThreads) dst[i] = from_acc<T>(to_acc<T>(src[i]) * f);
-  for (int i = tail + threadIdx.x; i < n; i += kClipThreads) dst[i] = from_acc<T>(to_acc<T>(src[i]) * f);
-  for (int v = threadIdx.x; v < nvec; v += kClipThreads * U) {
+  for (int i = me; i < head; i += threads) dst[i] = from_acc<T>(to_acc<T>(src[i]) * f);
+  for (int i = tail + me; i < n; i += threads) dst[i] = from_acc<T>(to_acc<T>(src[i]) * f);
+  for (int v = me; v < nvec; v += threads * U) {
     Raw<16> r[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = v + u * kClipThreads;
-      if (i < nvec) r[u] = ld_rw<16>(src + head + static_cast<int64_t>(i) * NV);
+      const int i = v + u * threads;
+      if (i < nvec) r[u] = ld_rw_hint<16>(src + head + static_cast<int64_t>(i) * NV, policy);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = v + u * kClipThreads;
+      const int i = v + u * threads;
       if (i < nvec) {
         A e[NV];
         expand<T, 16>(r[u], e);
 #pragma unroll
         for (int j = 0; j < NV; ++j) e[j] *= f;
-        st_row<16>(dst + head + static_cast<int64_t>(i) * NV, narrow<T, 16>(e));
+        st_row_hint<16>(dst + head + static_cast<int64_t>(i) * NV, narrow<T, 16>(e), policy);
       }
     }
   }
 }
 
+template <int U, int CAP>
+__device__ __forceinline__ void piece_scale(const Table<CAP>& t, const Piece& p, double f, int me, int threads, uint64_t policy) {
+  const void* src = t.src[p.tensor];
+  void* dst = t.dst[p.tensor];
+  switch (t.dtype[p.tensor]) {
+    case TBE_F16:
+      return scale_chunk<U>(static_cast<const __half*>(src) + p.at, static_cast<__half*>(dst) + p.at, p.n, f, me, threads, policy);
+    case TBE_BF16:
+      return scale_chunk<U>(static_cast<const __nv_bfloat16*>(src) + p.at, static_cast<__nv_bfloat16*>(dst) + p.at, p.n, f, me,
+                         threads, policy);
+    case TBE_F32:
+      return scale_chunk<U>(static_cast<const float*>(src) + p.at, static_cast<float*>(dst) + p.at, p.n, f, me, threads, policy);
+    default:
+      return scale_chunk<U>(static_cast<const double*>(src) + p.at, static_cast<double*>(dst) + p.at, p.n, f, me, threads, policy);
+  }
+}
+
+__device__ __forceinline__ double factor(double norm, double max_norm, double eps) {
+  const double f = max_norm / (norm + eps);
+  return f > 1.0 ? 1.0 : f;  // NaN stays
+}
+
 template <int CAP>
 __global__ void __launch_bounds__(kClipThreads) grad_scale_kernel(const __grid_constant__ Table<CAP> t, const double* partial,
-                                                                  int parts, double max_norm, double eps, bool in_place,
-                                                                  float* norm) {
-  const double n2 = fold(partial, parts);
-  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n2);
-  double f = max_norm / (n2 + eps);
-  if (f > 1.0) f = 1.0;  // NaN stays
+                                                                     int parts, double max_norm, double eps, bool in_place,
+                                                                     float* norm) {
+  const double n = fold(partial, parts);
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
+  const double f = factor(n, max_norm, eps);
   if (in_place && f == 1.0) return;
-  for (int c = t.chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {
-    const int k = tensor_of(t, c);
-    const int64_t at = static_cast<int64_t>(c - t.first[k]) * kChunk;
-    const int64_t left = t.n[k] - at;
-    const int n = static_cast<int>(left < kChunk ? left : kChunk);
-    switch (t.dtype[k]) {
-      case TBE_F16: scale_chunk(static_cast<const __half*>(t.src[k]) + at, static_cast<__half*>(t.dst[k]) + at, n, f); break;
-      case TBE_BF16:
-        scale_chunk(static_cast<const __nv_bfloat16*>(t.src[k]) + at, static_cast<__nv_bfloat16*>(t.dst[k]) + at, n, f);
-        break;
-      case TBE_F32: scale_chunk(static_cast<const float*>(t.src[k]) + at, static_cast<float*>(t.dst[k]) + at, n, f); break;
-      default: scale_chunk(static_cast<const double*>(t.src[k]) + at, static_cast<double*>(t.dst[k]) + at, n, f); break;
-    }
+  const uint64_t pass = l2_policy_evict_first();
+  for (int c = t.chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x)
+    piece_scale<4>(t, piece_of(t, c, kChunk), f, threadIdx.x, kClipThreads, pass);
+}
+
+// A short list in one launch: a cluster of CTAs, a warp per kSmallChunk elements, the CTAs' sums exchanged
+// through distributed shared memory between the two passes.
+template <int CAP>
+__global__ void __launch_bounds__(1024) grad_clip_small_kernel(const __grid_constant__ Table<CAP> t, bool scale, double max_norm,
+                                                               double eps, bool in_place, float* norm) {
+  __shared__ double part[32], own;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int first = static_cast<int>(cluster.block_rank()) * 32 + warp, step = kSmallCluster * 32;
+  const uint64_t policy = l2_policy_evict_normal();
+  double s = 0.0;
+  for (int c = first; c < t.chunks; c += step) s += piece_squares(t, piece_of(t, c, kSmallChunk), lane, 32, policy);
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) s += __shfl_xor_sync(kFullMask, s, m);
+  if (lane == 0) part[warp] = s;
+  __syncthreads();
+  if (warp == 0) {
+    s = part[lane];
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) s += __shfl_xor_sync(kFullMask, s, m);
+    if (lane == 0) own = s;
   }
+  cluster.sync();  // every CTA's sum is in place
+  double total = 0.0;
+#pragma unroll
+  for (int r = 0; r < kSmallCluster; ++r) total += *cluster.map_shared_rank(&own, r);
+  cluster.sync();  // nobody's sum is read any more
+  const double n = sqrt(total);
+  if (first == 0 && lane == 0) *norm = static_cast<float>(n);
+  const double f = factor(n, max_norm, eps);
+  if (!scale || (in_place && f == 1.0)) return;
+  for (int c = first; c < t.chunks; c += step) piece_scale<2>(t, piece_of(t, c, kSmallChunk), f, lane, 32, policy);
 }
 
 // One launch's worth of the list: tensors [from, to), at most CAP of them, empty ones left out.
 template <int CAP>
-bool fill(Table<CAP>& t, const void* const* src, void* const* dst, const int64_t* n, const int32_t* dtype, int from, int to) {
+bool fill(Table<CAP>& t, const void* const* src, void* const* dst, const int64_t* n, const int32_t* dtype, int from, int to,
+          int chunk) {
   t.count = 0;
   int64_t chunks = 0;
   for (int i = from; i < to; ++i) {
@@ -207,11 +279,25 @@ bool fill(Table<CAP>& t, const void* const* src, void* const* dst, const int64_t
     t.first[t.count] = static_cast<int32_t>(chunks);
     t.dtype[t.count] = static_cast<uint8_t>(dtype[i]);
     ++t.count;
-    chunks += (n[i] + kChunk - 1) / kChunk;
+    chunks += (n[i] + chunk - 1) / chunk;
     if (chunks > 0x7fff0000) return false;
   }
   t.chunks = static_cast<int32_t>(chunks);
   return true;
+}
+
+// The chunk from which the rest of the list fits into half of L2.
+template <int CAP>
+int first_kept_chunk(const Table<CAP>& t) {
+  int64_t room = device_l2_bytes() / 2;
+  int c = t.chunks;
+  for (int k = t.count - 1; k >= 0 && room > 0; --k) {
+    const int64_t bytes = kChunk * static_cast<int64_t>(any_elem_size(t.dtype[k])), n = c - t.first[k];
+    const int64_t fit = room / bytes;
+    c -= static_cast<int>(n < fit ? n : fit);
+    room = n <= fit ? room - n * bytes : 0;
+  }
+  return c;
 }
 
 int launch_grid(int64_t chunks) {
@@ -272,11 +358,11 @@ int norm_launches(const void* const* src, const int64_t* n, const int32_t* dtype
   int from = 0;
   do {
     const int to = count - from < CAP ? count : from + CAP;
-    TBE_REQUIRE(fill(t, src, nullptr, n, dtype, from, to), "tbe_grad_norm: too many elements");
+    TBE_REQUIRE(fill(t, src, nullptr, n, dtype, from, to, kChunk), "tbe_grad_norm: too many elements");
     const int grid = launch_grid(t.chunks);
     {
       KernelTimer timer("grad_norm_kernel", stream);
-      grad_norm_kernel<CAP><<<grid, kClipThreads, 0, stream>>>(t, partial + *parts);
+      grad_norm_kernel<CAP><<<grid, kClipThreads, 0, stream>>>(t, partial + *parts, to == count ? first_kept_chunk(t) : t.chunks);
     }
     TBE_CHECK_LAUNCH("grad_norm_kernel");
     *parts += grid;
@@ -294,7 +380,7 @@ int scale_launches(const void* const* src, void* const* dst, const int64_t* n, c
   int to = count;
   do {
     const int from = to > CAP ? (to - 1) / CAP * CAP : 0;
-    TBE_REQUIRE(fill(t, src, dst, n, dtype, from, to), "tbe_grad_clip: too many elements");
+    TBE_REQUIRE(fill(t, src, dst, n, dtype, from, to, kChunk), "tbe_grad_clip: too many elements");
     {
       KernelTimer timer("grad_scale_kernel", stream);
       grad_scale_kernel<CAP><<<launch_grid(t.chunks), kClipThreads, 0, stream>>>(t, partial, parts, max_norm, eps, in_place,
@@ -305,6 +391,43 @@ int scale_launches(const void* const* src, void* const* dst, const int64_t* n, c
     to = from;
   } while (to > 0);
   return TBE_OK;
+}
+
+// Whether the list is short enough for the one-kernel form.
+bool is_small(const int64_t* n, int64_t count) {
+  if (count > kLargeTable) return false;
+  int64_t total = 0;
+  for (int64_t i = 0; i < count; ++i) total += n[i];
+  return total <= kSmallMost;
+}
+
+template <int CAP>
+int small_launch(const void* const* src, void* const* dst, const int64_t* n, const int32_t* dtype, int count, bool scale,
+                 double max_norm, double eps, bool in_place, float* norm, cudaStream_t stream) {
+  Table<CAP> t;
+  fill(t, src, dst, n, dtype, 0, count, kSmallChunk);
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = kSmallCluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(kSmallCluster);
+  cfg.blockDim = dim3(1024);
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  {
+    KernelTimer timer("grad_clip_small_kernel", stream);
+    TBE_CUDA_TRY(cudaLaunchKernelEx(&cfg, grad_clip_small_kernel<CAP>, t, scale, max_norm, eps, in_place, norm));
+  }
+  TBE_CHECK_LAUNCH("grad_clip_small_kernel");
+  return TBE_OK;
+}
+int run_small(const void* const* src, void* const* dst, const int64_t* n, const int32_t* dtype, int count, bool scale,
+              double max_norm, double eps, bool in_place, float* norm, cudaStream_t stream) {
+  return count <= kSmallTable
+             ? small_launch<kSmallTable>(src, dst, n, dtype, count, scale, max_norm, eps, in_place, norm, stream)
+             : small_launch<kLargeTable>(src, dst, n, dtype, count, scale, max_norm, eps, in_place, norm, stream);
 }
 
 int64_t launches_of(int64_t count) { return count <= kLargeTable ? 1 : (count + kLargeTable - 1) / kLargeTable; }
@@ -321,15 +444,17 @@ extern "C" int64_t tbe_grad_norm_workspace_bytes(int64_t count) {
 
 namespace tbe {
 namespace {
-int run_norm(const char* who, const void* const* src, const int64_t* n, const int32_t* dtype, int64_t count, void* workspace,
-             int64_t workspace_bytes, int* parts, cudaStream_t stream) {
-  if (const int rc = check_list(who, src, n, dtype, count)) return rc;
+int check_workspace(const char* who, int64_t count, const void* workspace, int64_t workspace_bytes) {
   const int64_t need = tbe_grad_norm_workspace_bytes(count);
   if (workspace == nullptr || workspace_bytes < need)
     return fail(TBE_ERR_WORKSPACE_TOO_SMALL, "%s: workspace of %lld bytes, %lld needed", who,
                 static_cast<long long>(workspace_bytes), static_cast<long long>(need));
   TBE_REQUIRE(addr_bits(workspace) % 8 == 0, "%s: the workspace must be 8-byte aligned", who);
-  double* partial = static_cast<double*>(workspace);
+  return TBE_OK;
+}
+
+int run_norm(const void* const* src, const int64_t* n, const int32_t* dtype, int64_t count, double* partial, int* parts,
+             cudaStream_t stream) {
   return count <= kSmallTable ? norm_launches<kSmallTable>(src, n, dtype, static_cast<int>(count), partial, parts, stream)
                               : norm_launches<kLargeTable>(src, n, dtype, static_cast<int>(count), partial, parts, stream);
 }
@@ -341,9 +466,12 @@ extern "C" int tbe_grad_norm(const void* const* tensors, const int64_t* numels, 
   using namespace tbe;
   TBE_REQUIRE(norm, "tbe_grad_norm: null pointer argument");
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  if (const int rc = check_list("tbe_grad_norm", tensors, numels, dtypes, count)) return rc;
+  if (const int rc = check_workspace("tbe_grad_norm", count, workspace, workspace_bytes)) return rc;
+  if (is_small(numels, count))
+    return run_small(tensors, nullptr, numels, dtypes, static_cast<int>(count), false, 0.0, 0.0, false, norm, stream);
   int parts = 0;
-  if (const int rc = run_norm("tbe_grad_norm", tensors, numels, dtypes, count, workspace, workspace_bytes, &parts, stream))
-    return rc;
+  if (const int rc = run_norm(tensors, numels, dtypes, count, static_cast<double*>(workspace), &parts, stream)) return rc;
   {
     KernelTimer timer("grad_norm_finish_kernel", stream);
     grad_norm_finish_kernel<<<1, kClipThreads, 0, stream>>>(static_cast<const double*>(workspace), parts, norm);
@@ -368,9 +496,11 @@ extern "C" int tbe_grad_clip(const void* const* tensors, void* const* outputs, c
     in_place &= outputs[i] == tensors[i];
   }
   if (const int rc = check_apart(tensors, outputs, numels, dtypes, count)) return rc;
+  if (const int rc = check_workspace("tbe_grad_clip", count, workspace, workspace_bytes)) return rc;
+  if (is_small(numels, count))
+    return run_small(tensors, outputs, numels, dtypes, static_cast<int>(count), true, max_norm, eps, in_place, norm, stream);
   int parts = 0;
-  if (const int rc = run_norm("tbe_grad_clip", tensors, numels, dtypes, count, workspace, workspace_bytes, &parts, stream))
-    return rc;
+  if (const int rc = run_norm(tensors, numels, dtypes, count, static_cast<double*>(workspace), &parts, stream)) return rc;
   const double* partial = static_cast<const double*>(workspace);
   return count <= kSmallTable ? scale_launches<kSmallTable>(tensors, outputs, numels, dtypes, static_cast<int>(count), partial,
                                                             parts, max_norm, eps, in_place, norm, stream)
