@@ -10,9 +10,13 @@
 // A row belongs to a group of G = 2^g lanes (several rows per warp when E is small), each lane holds V
 // of its logits as sort keys that carry the value's order and the column: the larger key is the larger
 // logit, or the lower column of equal ones.  16-bit logits fit value and column into 32 bits, so a warp
-// finds a maximum in one redux; 32-bit ones take 64-bit keys and two.  A lane sorts its keys in runs of
-// eight (a 19-comparator network), so that each of the k rounds only compares the runs' heads and pops
-// one of them.  Nothing but the logits is read and nothing is kept for the backward, which recomputes the
+// finds a maximum in one redux; 32-bit ones take 64-bit keys and two.
+//
+// The k largest lie in the k lanes with the largest maxima.  With a warp per row those lanes are found
+// first, by k rounds over the lanes' maxima alone; their values are dealt to all lanes, C = k V / 32 each
+// (2 or 4), and k rounds over those give the choices.  Groups of fewer lanes, and a k V above 128, run the
+// rounds over all keys: sorted in runs of eight (a 19-comparator network), a round compares the runs' heads
+// and pops one.  (65536 rows of 256, k = 8: that takes 33 us.)  Nothing but the logits is read and nothing is kept for the backward, which recomputes the
 // row's maximum and sum from the logits when it needs them.
 //
 // Bound by instruction issue, not by HBM: 65536 rows of 256 bf16 logits are 33.5 MB (5 us).
@@ -38,8 +42,8 @@ struct Key16 {
   __device__ static __forceinline__ void pair(uint32_t x, int col0, int col1, type* key) {
     const uint32_t sign = (x >> 15) & 0x00010001u;
     const uint32_t o = x ^ (0x80008000u | (sign * 0x7fffu));  // all bits of a negative, the top bit of the others
-    key[0] = (o << 16) | static_cast<uint32_t>(0xffff - col0);
-    key[1] = (o & 0xffff0000u) | static_cast<uint32_t>(0xffff - col1);
+    key[0] = __byte_perm(o, static_cast<uint32_t>(0xffff - col0), 0x1054);
+    key[1] = __byte_perm(o, static_cast<uint32_t>(0xffff - col1), 0x3254);
   }
   __device__ static __forceinline__ uint16_t bits(type k) {
     const uint32_t o = k >> 16;
@@ -167,6 +171,68 @@ __device__ __forceinline__ void sort8(K* k) {
   order2(k[1], k[2]), order2(k[3], k[4]), order2(k[5], k[6]);
 }
 
+// Rounds over C keys per lane in descending order: the k largest of the group, the s-th in lane s.
+// first(m) is called with the largest.
+template <int C, typename K, typename F>
+__device__ __forceinline__ K take_largest(K* key, int k, int sub, int glog, F first) {
+  constexpr int RUN = C < 8 ? C : 8;  // the keys come in sorted runs
+  K mine = 0;
+  for (int s = 0; s < k; ++s) {
+    K m = key[0];
+#pragma unroll
+    for (int r = RUN; r < C; r += RUN) m = key[r] > m ? key[r] : m;
+    m = group_max(m, glog);
+    if (s == 0) first(m);
+    if (sub == s) mine = m;
+#pragma unroll
+    for (int r = 0; r < C; r += RUN) {
+      const bool pop = key[r] == m;
+#pragma unroll
+      for (int i = r; i < r + RUN - 1; ++i) key[i] = pop ? key[i + 1] : key[i];
+      key[r + RUN - 1] = pop ? K(0) : key[r + RUN - 1];
+    }
+  }
+  return mine;
+}
+
+// A warp per row: the keys of the k lanes with the largest maxima, dealt to the lanes through `room`
+// (32 * C keys of shared memory), then the rounds over those.
+template <int V, int C, typename K, typename F>
+__device__ __forceinline__ K take_from_best_lanes(const K* key, int k, int lane, K* room, F first) {
+  K best = key[0];
+#pragma unroll
+  for (int i = 1; i < V; ++i) best = key[i] > best ? key[i] : best;
+  int rank = -1, lanes = 0;
+  for (int s = 0; s < k; ++s) {
+    const K m = group_max(best, 5);
+    if (s == 0) first(m);
+    if (m == K(0)) break;  // (the whole warp) no candidate is left
+    lanes = s + 1;
+    if (best == m) {  // keys differ: one lane
+      rank = s;
+      best = 0;
+    }
+  }
+  // lanes * V keys are written, in 16-byte stores; a lane behind them has nothing
+  struct alignas(16) Some {
+    K key[V];
+  } all;
+  struct alignas(C * sizeof(K) < 16 ? C * sizeof(K) : 16) Few {
+    K key[C];
+  } mine;
+#pragma unroll
+  for (int i = 0; i < V; ++i) all.key[i] = key[i];
+  if (rank >= 0) reinterpret_cast<Some*>(room)[rank] = all;
+  __syncwarp();
+  mine = reinterpret_cast<const Few*>(room)[lane];
+  K few[C];
+#pragma unroll
+  for (int i = 0; i < C; ++i) few[i] = lane * C < lanes * V ? mine.key[i] : K(0);
+  order2(few[0], few[1]);
+  if (C == 4) order2(few[2], few[3]), order2(few[0], few[2]), order2(few[1], few[3]), order2(few[1], few[2]);
+  return take_largest<C>(few, k, lane, 5, [](K) {});
+}
+
 // Column of a lane's i-th value: vectors of VE neighbouring columns, dealt to the lanes in turn.
 template <int VE>
 __device__ __forceinline__ int column(int i, int sub, int glog) {
@@ -202,11 +268,12 @@ struct GateArgs {
   void* grad_logits;
 };
 
-template <typename T, int V, int VE>
+// WARP: a warp per row (a.glog is 5), known at compile time.
+template <typename T, int V, int VE, bool WARP>
 __global__ void __launch_bounds__(kGateThreads) gate_kernel(GateArgs a) {
   using A = typename Acc<T>::type;
   using K = typename Key<T>::type;
-  const int lane = threadIdx.x & 31, glog = a.glog, sub = lane & ((1 << glog) - 1);
+  const int lane = threadIdx.x & 31, glog = WARP ? 5 : a.glog, sub = lane & ((1 << glog) - 1);
   const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kGateThreads >> 5) + (threadIdx.x >> 5);
   const int64_t row = (warp << (5 - glog)) + (lane >> glog);
   const bool live = row < a.N;
@@ -215,35 +282,34 @@ __global__ void __launch_bounds__(kGateThreads) gate_kernel(GateArgs a) {
   K key[V];
 #pragma unroll
   for (int i = 0; i < V; i += 2) Key<T>::of(v + i, column<VE>(i, sub, glog), column<VE>(i + 1, sub, glog), key + i);
-#pragma unroll
-  for (int r = 0; r < V; r += 8) sort8(key + r);
-
-  K mine = 0;  // the s-th largest, in lane s of the group (k <= G)
   A top = 0, sum = 0;
-  for (int s = 0; s < a.k; ++s) {
-    K m = key[0];
-#pragma unroll
-    for (int r = 8; r < V; r += 8) m = key[r] > m ? key[r] : m;
-    m = group_max(m, glog);
-    if (s == 0 && !a.renormalize) {
-      top = Key<T>::alive(m) ? Key<T>::value(m) : A(0);
+  auto first = [&](K m) {
+    top = Key<T>::alive(m) ? Key<T>::value(m) : A(0);
+    if (!a.renormalize) {
 #pragma unroll
       for (int i = 0; i < V; ++i) sum += exp(to_acc<T>(v[i]) - top);  // -inf adds 0
     }
-    if (s == 0 && a.renormalize) top = Key<T>::alive(m) ? Key<T>::value(m) : A(0);
-    if (sub == s) mine = m;
+  };
+  __shared__ __align__(16) K room[kGateThreads / 32][128];
+  K mine;  // the s-th largest, in lane s of the group (k <= G)
+  if (WARP && a.k * V <= 64) {
+    mine = take_from_best_lanes<V, 2>(key, a.k, lane, room[threadIdx.x >> 5], first);
+  } else if (WARP && a.k * V <= 128) {
+    mine = take_from_best_lanes<V, 4>(key, a.k, lane, room[threadIdx.x >> 5], first);
+  } else {
 #pragma unroll
-    for (int r = 0; r < V; r += 8) {
-      const bool pop = key[r] == m;
-#pragma unroll
-      for (int i = r; i < r + 7; ++i) key[i] = pop ? key[i + 1] : key[i];
-      key[r + 7] = pop ? K(0) : key[r + 7];
-    }
+    for (int r = 0; r < V; r += 8) sort8(key + r);
+    mine = take_largest<V>(key, a.k, sub, glog, first);
   }
   const bool chosen = sub < a.k && Key<T>::alive(mine);
   const A e = chosen ? exp(Key<T>::value(mine) - top) : A(0);
   if (a.renormalize) sum = e;
-  sum = group_sum(sum, glog);
+  if (WARP) {
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) sum += __shfl_xor_sync(kFullMask, sum, m);
+  } else {
+    sum = group_sum(sum, glog);
+  }
   if (live && sub < a.k) {
     const int64_t at = row * a.k + sub;
     a.experts[at] = chosen ? Key<T>::col(mine) : -1;
@@ -332,7 +398,8 @@ int launch_gate(const GateArgs& a, bool backward, cudaStream_t stream) {
   if (blocks > 0x7fffffff) return fail(TBE_ERR_INVALID_ARGUMENT, "tbe_expert_gate: too many rows");
   if (!backward) {
     KernelTimer timer("gate_kernel", stream);
-    gate_kernel<T, V, VE><<<static_cast<unsigned>(blocks), kGateThreads, 0, stream>>>(a);
+    if (a.glog == 5) gate_kernel<T, V, VE, true><<<static_cast<unsigned>(blocks), kGateThreads, 0, stream>>>(a);
+    else if constexpr (V == 8) gate_kernel<T, V, VE, false><<<static_cast<unsigned>(blocks), kGateThreads, 0, stream>>>(a);
   } else {
     KernelTimer timer("gate_backward_kernel", stream);
     const size_t shared = sizeof(typename Acc<T>::type) * kGateThreads * V;  // at most 64 KB (fp64, V = 32)

@@ -24,7 +24,8 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kClipThreads = 256;
-constexpr int kClipBlocksPerSM = 8;
+constexpr int kClipBlocksPerSM = 8;   // norm pass (32 registers)
+constexpr int kScaleBlocksPerSM = 3;  // scaling pass (80): all resident, or the sweep would not run backwards
 constexpr int kChunk = 16384;      // elements
 constexpr int kSmallChunk = 1024;  // elements per warp of the one-kernel form
 constexpr int kSmallMost = 1 << 18;
@@ -219,7 +220,7 @@ __device__ __forceinline__ double factor(double norm, double max_norm, double ep
 }
 
 template <int CAP>
-__global__ void __launch_bounds__(kClipThreads) grad_scale_kernel(const __grid_constant__ Table<CAP> t, const double* partial,
+__global__ void __launch_bounds__(kClipThreads, kScaleBlocksPerSM) grad_scale_kernel(const __grid_constant__ Table<CAP> t, const double* partial,
                                                                      int parts, double max_norm, double eps, bool in_place,
                                                                      float* norm) {
   const double n = fold(partial, parts);
@@ -300,8 +301,8 @@ int first_kept_chunk(const Table<CAP>& t) {
   return c;
 }
 
-int launch_grid(int64_t chunks) {
-  const int64_t most = static_cast<int64_t>(device_sm_count()) * kClipBlocksPerSM;
+int launch_grid(int64_t chunks, int blocks_per_sm) {
+  const int64_t most = static_cast<int64_t>(device_sm_count()) * blocks_per_sm;
   return static_cast<int>(chunks < most ? (chunks > 0 ? chunks : 1) : most);
 }
 
@@ -359,7 +360,7 @@ int norm_launches(const void* const* src, const int64_t* n, const int32_t* dtype
   do {
     const int to = count - from < CAP ? count : from + CAP;
     TBE_REQUIRE(fill(t, src, nullptr, n, dtype, from, to, kChunk), "tbe_grad_norm: too many elements");
-    const int grid = launch_grid(t.chunks);
+    const int grid = launch_grid(t.chunks, kClipBlocksPerSM);
     {
       KernelTimer timer("grad_norm_kernel", stream);
       grad_norm_kernel<CAP><<<grid, kClipThreads, 0, stream>>>(t, partial + *parts, to == count ? first_kept_chunk(t) : t.chunks);
@@ -383,7 +384,7 @@ int scale_launches(const void* const* src, void* const* dst, const int64_t* n, c
     TBE_REQUIRE(fill(t, src, dst, n, dtype, from, to, kChunk), "tbe_grad_clip: too many elements");
     {
       KernelTimer timer("grad_scale_kernel", stream);
-      grad_scale_kernel<CAP><<<launch_grid(t.chunks), kClipThreads, 0, stream>>>(t, partial, parts, max_norm, eps, in_place,
+      grad_scale_kernel<CAP><<<launch_grid(t.chunks, kScaleBlocksPerSM), kClipThreads, 0, stream>>>(t, partial, parts, max_norm, eps, in_place,
                                                                                  norm);
     }
     TBE_CHECK_LAUNCH("grad_scale_kernel");
