@@ -337,11 +337,12 @@ __global__ void __launch_bounds__(kGateThreads) gate_backward_kernel(GateArgs a)
   int col = -1;
   if (live && sub < a.k) {
     const int64_t at = row * a.k + sub;
-    col = a.experts[at];
-    if (col >= a.E) col = -1;
-    if (col >= 0) {
-      w = static_cast<const A*>(a.weights)[at];
-      g = static_cast<const A*>(a.grad_weights)[at];
+    col = a.experts[at];  // (three independent loads)
+    w = static_cast<const A*>(a.weights)[at];
+    g = static_cast<const A*>(a.grad_weights)[at];
+    if (col < 0 || col >= a.E) {
+      col = -1;
+      w = g = A(0);
     }
   }
   const A c = group_sum(w * g, glog);

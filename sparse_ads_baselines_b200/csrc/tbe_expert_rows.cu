@@ -56,8 +56,10 @@ __device__ void block_exclusive_scan(int32_t* v, int n, int32_t* warp_sums) {
   }
   if (lane == 31) warp_sums[warp] = scan;
   __syncthreads();
-  int32_t before = scan - own;
-  for (int w = 0; w < warp; ++w) before += warp_sums[w];
+  int32_t ws = lane < warp ? warp_sums[lane] : 0;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) ws += __shfl_xor_sync(kFullMask, ws, m);
+  int32_t before = scan - own + ws;
   for (int i = begin; i < end; ++i) {
     const int32_t x = v[i];
     v[i] = before;
@@ -86,6 +88,7 @@ __global__ void __launch_bounds__(1024) plan_place_kernel(PlanArgs a) {
 
   for (int i = threadIdx.x; i < warps * E1 + 2 * E1; i += blockDim.x) hist[i] = 0;
   __syncthreads();
+#pragma unroll 4
   for (int i = wb + lane; i < we; i += 32) atomicAdd(&hist[warp * E1 + bin_of(__ldg(a.experts + i), a.E)], 1);
   if (MODE == kGrid) {
     const int n = gridDim.x * E1, mine = blockIdx.x * E1;
@@ -101,10 +104,15 @@ __global__ void __launch_bounds__(1024) plan_place_kernel(PlanArgs a) {
   __syncthreads();
   for (int b = threadIdx.x; b < E1; b += blockDim.x) {
     int32_t run = 0;
-    for (int w = 0; w < warps; ++w) {
-      const int32_t c = hist[w * E1 + b];
-      hist[w * E1 + b] = run;
-      run += c;
+    for (int w0 = 0; w0 < warps; w0 += 8) {  // (warps is a multiple of 8)
+      int32_t c[8];
+#pragma unroll
+      for (int w = 0; w < 8; ++w) c[w] = hist[(w0 + w) * E1 + b];
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        hist[(w0 + w) * E1 + b] = run;
+        run += c[w];
+      }
     }
     if (MODE == kOne) start[b] = run;
     if (MODE == kCluster) own[b] = run;
@@ -138,10 +146,12 @@ __global__ void __launch_bounds__(1024) plan_place_kernel(PlanArgs a) {
   }
 
   int32_t* next = hist + warp * E1;
+  int32_t ahead = wb + lane < we ? __ldg(a.experts + wb + lane) : 0;
   for (int i0 = wb; i0 < we; i0 += 32) {
     const int i = i0 + lane;
     const bool on = i < we;
-    const int b = on ? bin_of(__ldg(a.experts + i), a.E) : E1;
+    const int b = on ? bin_of(ahead, a.E) : E1;
+    if (i + 32 < we) ahead = __ldg(a.experts + i + 32);
     const unsigned peers = __match_any_sync(kFullMask, b);
     const int rank = __popc(peers & ((1u << lane) - 1));
     const int32_t first = on ? next[b] : 0;
@@ -417,7 +427,7 @@ int launch_dispatch(const RowArgs& a, int64_t N, cudaStream_t stream) {
 template <typename T, int VB, int KB>
 int launch_combine_k(const RowArgs& a, int64_t N, cudaStream_t stream) {
   using A = typename Acc<T>::type;
-  constexpr int U = vectors_per_thread(VB);
+  constexpr int U = vectors_per_thread(VB) * (KB == 2 ? 2 : 1);  // at least four 16-byte loads in flight
   return per_sample_launches("combine_kernel", a, N, VB, U, stream, [&](int64_t n0, RowArgs b, unsigned blocks) {
     b.weights = a.weights ? static_cast<const A*>(a.weights) + n0 * a.k : nullptr;
     b.out = a.out + n0 * a.row_bytes;

@@ -287,7 +287,8 @@ bool fill(Table<CAP>& t, const void* const* src, void* const* dst, const int64_t
   return true;
 }
 
-// The chunk from which the rest of the list fits into half of L2.
+// The chunk from which the rest of the list fits into half of L2.  (200 M bf16 elements, norm + scaling:
+// 67 + 127 us with nothing kept, 68 + 122 with 63 MB, 71 + 120 with 126 MB, 79 + 120 with everything.)
 template <int CAP>
 int first_kept_chunk(const Table<CAP>& t) {
   int64_t room = device_l2_bytes() / 2;
