@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <new>
+#include <utility>
 
 #include "tbe_elem.cuh"
 
@@ -119,9 +120,9 @@ struct Piece {
   int n;
 };
 template <int CAP>
-__device__ __forceinline__ Piece piece_of(const Table<CAP>& t, int c, int chunk) {
+__device__ __forceinline__ Piece piece_of(const Table<CAP>& t, int c, int chunk, int tensor) {
   Piece p;
-  p.tensor = tensor_of(t, c);
+  p.tensor = tensor;
   p.at = static_cast<int64_t>(c - t.first[p.tensor]) * chunk;
   const int64_t left = t.n[p.tensor] - p.at;
   p.n = static_cast<int>(left < chunk ? left : chunk);
@@ -145,7 +146,7 @@ __global__ void __launch_bounds__(kClipThreads) grad_norm_kernel(const __grid_co
   const uint64_t pass = l2_policy_evict_first(), stay = l2_policy_evict_normal();
   double s = 0.0;
   for (int c = blockIdx.x; c < t.chunks; c += gridDim.x)
-    s += piece_squares(t, piece_of(t, c, kChunk), threadIdx.x, kClipThreads, c < keep ? pass : stay);
+    s += piece_squares(t, piece_of(t, c, kChunk, tensor_of(t, c)), threadIdx.x, kClipThreads, c < keep ? pass : stay);
   s = block_sum(s);
   if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
@@ -167,13 +168,12 @@ __device__ void scale_chunk(const T* src, T* dst, int n, double c, int me, int t
   constexpr int NV = 16 / sizeof(T);
   const A f = static_cast<A>(c);
   const uintptr_t s = reinterpret_cast<uintptr_t>(src), d = reinterpret_cast<uintptr_t>(dst);
-  int head = min(n, static_cast<int>((16 - (s & 15)) & 15) / static_cast<int>(sizeof(T)));
-  int nvec = (n - head) / NV;
   if ((s ^ d) & 15) {  // no vector of one is a vector of the other
-    head = n;
-    nvec = 0;
+    for (int i = me; i < n; i += threads) dst[i] = from_acc<T>(to_acc<T>(src[i]) * f);
+    return;
   }
-  const int tail = head + nvec * NV;
+  const int head = min(n, static_cast<int>((16 - (s & 15)) & 15) / static_cast<int>(sizeof(T)));
+  const int nvec = (n - head) / NV, tail = head + nvec * NV;
   for (int i = me; i < head; i += threads) dst[i] = from_acc<T>(to_acc<T>(src[i]) * f);
   for (int i = tail + me; i < n; i += threads) dst[i] = from_acc<T>(to_acc<T>(src[i]) * f);
   for (int v = me; v < nvec; v += threads * U) {
@@ -187,11 +187,11 @@ __device__ void scale_chunk(const T* src, T* dst, int n, double c, int me, int t
     for (int u = 0; u < U; ++u) {
       const int i = v + u * threads;
       if (i < nvec) {
-        A e[NV];
-        expand<T, 16>(r[u], e);
+        A x[NV];
+        expand<T, 16>(r[u], x);
 #pragma unroll
-        for (int j = 0; j < NV; ++j) e[j] *= f;
-        st_row_hint<16>(dst + head + static_cast<int64_t>(i) * NV, narrow<T, 16>(e), policy);
+        for (int j = 0; j < NV; ++j) x[j] *= f;
+        st_row_hint<16>(dst + head + static_cast<int64_t>(i) * NV, narrow<T, 16>(x), policy);
       }
     }
   }
@@ -229,21 +229,35 @@ __global__ void __launch_bounds__(kClipThreads, kScaleBlocksPerSM) grad_scale_ke
   if (in_place && f == 1.0) return;
   const uint64_t pass = l2_policy_evict_first();
   for (int c = t.chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x)
-    piece_scale<4>(t, piece_of(t, c, kChunk), f, threadIdx.x, kClipThreads, pass);
+    piece_scale<4>(t, piece_of(t, c, kChunk, tensor_of(t, c)), f, threadIdx.x, kClipThreads, pass);
 }
+
+// The tensor of every chunk of a short list: in a kernel of a few microseconds a search in the table is a
+// chain of loads that all miss the constant cache.
+template <int CAP>
+struct Owners {
+  uint16_t tensor[CAP + kSmallMost / kSmallChunk];
+};
 
 // A short list in one launch: a cluster of CTAs, a warp per kSmallChunk elements, the CTAs' sums exchanged
 // through distributed shared memory between the two passes.
 template <int CAP>
-__global__ void __launch_bounds__(1024) grad_clip_small_kernel(const __grid_constant__ Table<CAP> t, bool scale, double max_norm,
-                                                               double eps, bool in_place, float* norm) {
+__global__ void __launch_bounds__(1024) grad_clip_small_kernel(const __grid_constant__ Table<CAP> t,
+                                                               const __grid_constant__ Owners<CAP> owners, bool scale,
+                                                               double max_norm, double eps, bool in_place, float* norm) {
   __shared__ double part[32], own;
   cg::cluster_group cluster = cg::this_cluster();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int first = static_cast<int>(cluster.block_rank()) * 32 + warp, step = kSmallCluster * 32;
   const uint64_t policy = l2_policy_evict_normal();
   double s = 0.0;
-  for (int c = first; c < t.chunks; c += step) s += piece_squares(t, piece_of(t, c, kSmallChunk), lane, 32, policy);
+  Piece own_piece{0, 0, 0};  // the first of this warp's pieces, which is all it has unless the list is long
+  if (first < t.chunks) {
+    own_piece = piece_of(t, first, kSmallChunk, owners.tensor[first]);
+    s = piece_squares(t, own_piece, lane, 32, policy);
+  }
+  for (int c = first + step; c < t.chunks; c += step)
+    s += piece_squares(t, piece_of(t, c, kSmallChunk, owners.tensor[c]), lane, 32, policy);
 #pragma unroll
   for (int m = 1; m < 32; m <<= 1) s += __shfl_xor_sync(kFullMask, s, m);
   if (lane == 0) part[warp] = s;
@@ -258,12 +272,16 @@ __global__ void __launch_bounds__(1024) grad_clip_small_kernel(const __grid_cons
   double total = 0.0;
 #pragma unroll
   for (int r = 0; r < kSmallCluster; ++r) total += *cluster.map_shared_rank(&own, r);
-  cluster.sync();  // nobody's sum is read any more
+  auto read = cluster.barrier_arrive();  // this CTA has read the others' sums
   const double n = sqrt(total);
   if (first == 0 && lane == 0) *norm = static_cast<float>(n);
   const double f = factor(n, max_norm, eps);
-  if (!scale || (in_place && f == 1.0)) return;
-  for (int c = first; c < t.chunks; c += step) piece_scale<2>(t, piece_of(t, c, kSmallChunk), f, lane, 32, policy);
+  if (scale && !(in_place && f == 1.0)) {
+    if (first < t.chunks) piece_scale<2>(t, own_piece, f, lane, 32, policy);
+    for (int c = first + step; c < t.chunks; c += step)
+      piece_scale<2>(t, piece_of(t, c, kSmallChunk, owners.tensor[c]), f, lane, 32, policy);
+  }
+  cluster.barrier_wait(std::move(read));  // nobody reads a CTA's sum after it has left
 }
 
 // One launch's worth of the list: tensors [from, to), at most CAP of them, empty ones left out.
@@ -407,7 +425,11 @@ template <int CAP>
 int small_launch(const void* const* src, void* const* dst, const int64_t* n, const int32_t* dtype, int count, bool scale,
                  double max_norm, double eps, bool in_place, float* norm, cudaStream_t stream) {
   Table<CAP> t;
-  fill(t, src, dst, n, dtype, 0, count, kSmallChunk);
+  Owners<CAP> owners;
+  static_assert(sizeof(t) + sizeof(owners) + 64 <= 32764, "the tables do not fit into a kernel's parameters");
+  fill(t, src, dst, n, dtype, 0, count, kSmallChunk);  // at most CAP + kSmallMost / kSmallChunk chunks
+  for (int k = 0; k < t.count; ++k)
+    for (int c = t.first[k]; c < (k + 1 < t.count ? t.first[k + 1] : t.chunks); ++c) owners.tensor[c] = static_cast<uint16_t>(k);
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = kSmallCluster;
@@ -420,7 +442,7 @@ int small_launch(const void* const* src, void* const* dst, const int64_t* n, con
   cfg.numAttrs = 1;
   {
     KernelTimer timer("grad_clip_small_kernel", stream);
-    TBE_CUDA_TRY(cudaLaunchKernelEx(&cfg, grad_clip_small_kernel<CAP>, t, scale, max_norm, eps, in_place, norm));
+    TBE_CUDA_TRY(cudaLaunchKernelEx(&cfg, grad_clip_small_kernel<CAP>, t, owners, scale, max_norm, eps, in_place, norm));
   }
   TBE_CHECK_LAUNCH("grad_clip_small_kernel");
   return TBE_OK;

@@ -143,8 +143,8 @@ def test_gate_gradcheck(cuda_device):
 
 # ---------------------------------------------------------------------------- plan
 
-@pytest.mark.parametrize("N,k", [(0, 3), (1, 1), (1, 8), (7, 1), (128, 8), (129, 8), (1024, 8), (1025, 8), (2731, 3),
-                                 (20000, 2), (50001, 7), (200000, 8)])
+@pytest.mark.parametrize("N,k", [(0, 3), (1, 1), (1, 8), (7, 1), (128, 8), (129, 8), (512, 8), (4097, 1), (1025, 8),
+                                 (2731, 3), (20000, 2), (16384, 8), (131073, 1), (50001, 7), (200000, 8)])
 @pytest.mark.parametrize("E", [1, 2, 61, 256, 1024])
 def test_plan(cuda_device, N, k, E):
     rng = np.random.default_rng(N + k + E)
@@ -344,6 +344,24 @@ def test_past_32_bit_offsets(cuda_device):
             assert torch.equal(dw[t:n], x[t:n].float().square().sum(1, keepdim=True).expand(-1, k))
         del x, y, out, dy, dw, w
         torch.cuda.empty_cache()
+
+
+def test_several_launches(cuda_device):
+    """Calls beyond 2^32 threads are cut by samples; the knob makes small ones take the same way."""
+    from sparse_ads_baselines_b200 import _lib
+    for D, dtype in ((64, torch.bfloat16), (33, torch.float32)):
+        rng, p, _, _ = _cases(100, 3, 8, D, dtype, 0.2, cuda_device)
+        x = _randn(rng, (100, D + 3), dtype, cuda_device)[:, 1:D + 1]
+        y = _randn(rng, (300, D), dtype, cuda_device)
+        w = _randn(rng, (100, 3), torch.float32, cuda_device)
+        a, b, c = er.dispatch(x, p), er.combine(y, p, w), er.combine(y, p)
+        try:
+            for most in (1, 7, 100, 333):
+                _lib.call("tbe_set_tuning", b"row_threads", most)
+                assert torch.equal(er.dispatch(x, p), a) and torch.equal(er.combine(y, p, w), b)
+                assert torch.equal(er.combine(y, p), c)
+        finally:
+            _lib.call("tbe_set_tuning", b"row_threads", 0)
 
 
 # ---------------------------------------------------------------------------- streams, graphs, repeats

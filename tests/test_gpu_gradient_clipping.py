@@ -79,6 +79,19 @@ def test_many_tensors_of_mixed_types(cuda_device, count):
     assert abs(float(gc.grad_norm(mixed)) - _norm([t for t in mixed if t is not None])) <= NORM_TOL * float(norm)
 
 
+@pytest.mark.parametrize("sizes", [[2 ** 18], [2 ** 18 + 1], [2 ** 18 - 64] + [1] * 64, [255] * 1000, [2000] * 130,
+                                   [10 ** 6] + [3] * 70], ids=["one", "one more", "65", "1000", "130", "71"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=name)
+def test_around_the_one_kernel_limit(cuda_device, sizes, dtype):
+    before = _make(sizes, dtype, cuda_device)
+    g = [t.clone() for t in before]
+    norm = gc.clip_grad_norm(g, 7.0)
+    _check(before, g, norm, 7.0)
+    assert torch.equal(gc.grad_norm(before), norm)
+    assert torch.equal(gc.clip_grad_norm(before, float("inf")), norm)  # nothing to do: the same bits again
+    assert torch.equal(gc.grad_norm(before), norm)
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=name)
 def test_views_of_a_bucket_at_any_alignment(cuda_device, dtype):
     """Neighbouring views; what lies between and around them keeps its bytes."""
