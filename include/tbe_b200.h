@@ -305,7 +305,7 @@ TBE_API int tbe_sort_segments(const int32_t* table_offsets, const int32_t* indic
 /* For models whose samples pass through a few of E experts.  The reference has no such layer.  dtype is
  * any tbe_dtype_t; "weights" and their gradients are fp32 (fp64 for TBE_F64).  All arrays are device
  * memory.  Rows may have any width; they move in the widest vectors (16 bytes down to one element) that
- * the addresses and strides allow.  Limits: E <= 1024, k <= min(E, 32) in the gate, N*k < 2^31.
+ * the addresses and strides allow.  Limits: E <= 1024, k <= min(E, 32) in the gate, N*k <= 2^31 - 1025.
  *
  * tbe_expert_gate: logits [N][E] (rows row_stride elements apart) -> the k largest of every row,
  * descending, ties to the lowest index: experts int32 [N][k], and weights [N][k]:
@@ -322,7 +322,8 @@ TBE_API int tbe_expert_gate_backward(const void* grad_weights, const void* logit
 /* Stable sort of M choices (experts[M] = [N][k] flattened) by expert: positions[i] is the row choice i
  * takes, order[positions[i]] = i, and rows offsets[e] .. offsets[e+1) (int32 [E+1]) are expert e's.  Ids
  * outside 0..E-1 -- unassigned slots, experts of another rank -- sort behind all experts, at rows
- * offsets[E] .. M-1.  One kernel for up to 131072 choices, two above (workspace:
+ * offsets[E] .. M-1.  The calls below take any such permutation; a position outside 0..M-1 is skipped,
+ * one that stands twice leaves a row of an output unwritten.  One kernel for up to 131072 choices, two above (workspace:
  * tbe_expert_plan_workspace_bytes, 0 for one kernel; it needs no initialisation). */
 TBE_API int64_t tbe_expert_plan_workspace_bytes(int64_t M, int64_t E);
 TBE_API int tbe_expert_plan(const int32_t* experts, int32_t* offsets, int32_t* positions, int32_t* order, int64_t M,
@@ -346,8 +347,8 @@ TBE_API int tbe_expert_combine_backward(const void* grad_out, int64_t grad_strid
 
 /* ---- gradients: global norm and clipping ----------------------------------- */
 
-/* norm (device, one float) = sqrt(sum of squares over all elements of `count` tensors), summed in fp64 in
- * a fixed order.  tensors, numels and dtypes are HOST arrays, read during the call; every tensor is dense
+/* norm (device, one float; inf where it passes fp32's range) = sqrt(sum of squares over all elements of
+ * `count` tensors), summed in fp64 in a fixed order.  tensors, numels and dtypes are HOST arrays, read during the call; every tensor is dense
  * memory of numels[i] elements (0 is allowed) on the current device.  The table travels in the kernels'
  * parameters, 1024 tensors per launch. */
 TBE_API int64_t tbe_grad_norm_workspace_bytes(int64_t count);

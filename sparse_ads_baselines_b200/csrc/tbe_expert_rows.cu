@@ -21,6 +21,7 @@ namespace tbe {
 namespace {
 
 constexpr int kMaxExperts = 1024;
+constexpr int64_t kMaxEntries = 0x7fffffffll - 1024;  // 32-bit positions, and room for an index past the end
 namespace cg = cooperative_groups;
 
 // How many CTAs sort a plan, by its number of choices: one, one cluster (totals exchanged through
@@ -389,7 +390,8 @@ __global__ void __launch_bounds__(G == 128 ? 128 : 256) combine_backward_kernel(
 
 // ---------------------------------------------------------------- launches
 // Vectors per thread: 16 bytes' worth, so that narrow vectors have as many loads in flight as wide ones.
-// (5003 rows of 1001 fp32 values, six choices each: one 4-byte vector a thread moved 3.6 and 3.0 TB/s.)
+// (Combining 5003 rows of 1001 fp32 values, six choices each: 43 us with one 4-byte vector a thread, 34 with
+// two or four, 95 with eight.  dispatch has its k stores as well: 35 us with one, 29 with two, 30 with four.)
 constexpr int vectors_per_thread(int vb) { return vb == 16 ? 1 : vb == 8 ? 2 : 4; }
 
 // 32-bit thread indices: a launch covers as many samples as fit below 2^32 threads.  body(first sample,
@@ -417,7 +419,7 @@ int per_sample_launches(const char* name, RowArgs a, int64_t N, int vb, int u, c
 
 template <int VB>
 int launch_dispatch(const RowArgs& a, int64_t N, cudaStream_t stream) {
-  constexpr int U = 2 * vectors_per_thread(VB);
+  constexpr int U = VB == 2 ? 4 : 2;
   return per_sample_launches("dispatch_kernel", a, N, VB, U, stream, [&](int64_t n0, RowArgs b, unsigned blocks) {
     b.x = a.x + n0 * a.x_stride;
     dispatch_kernel<VB, U><<<blocks, 256, 0, stream>>>(b);
@@ -499,8 +501,8 @@ int launch_backward_type(const GradArgs& a, int vb, cudaStream_t stream) {
 
 int check_rows(const char* who, int64_t N, int64_t k, int64_t D, int dtype) {
   TBE_REQUIRE(known_dtype(dtype), "%s: bad dtype %d", who, dtype);
-  TBE_REQUIRE(N >= 0 && k > 0 && D > 0 && N < (1ll << 31) && k < (1ll << 31) && N * k < (1ll << 31),
-              "%s: N must be >= 0, k and D > 0, and N*k < 2^31", who);
+  TBE_REQUIRE(N >= 0 && k > 0 && D > 0 && N <= kMaxEntries && k <= kMaxEntries && N * k <= kMaxEntries,
+              "%s: N must be >= 0, k and D > 0, and N*k <= 2^31-1025", who);
   TBE_REQUIRE(D <= (1ll << 28), "%s: rows of more than 2^28 elements are not supported", who);
   return TBE_OK;
 }
@@ -510,8 +512,8 @@ int check_rows(const char* who, int64_t N, int64_t k, int64_t D, int dtype) {
 
 extern "C" int64_t tbe_expert_plan_workspace_bytes(int64_t M, int64_t E) {
   using namespace tbe;
-  if (M < 0 || M >= (1ll << 31) || E < 1 || E > kMaxExperts)
-    return fail(TBE_ERR_INVALID_ARGUMENT, "tbe_expert_plan_workspace_bytes: M must be 0..2^31-1 and E 1..%d", kMaxExperts);
+  if (M < 0 || M > kMaxEntries || E < 1 || E > kMaxExperts)
+    return fail(TBE_ERR_INVALID_ARGUMENT, "tbe_expert_plan: M must be 0..2^31-1025 and E 1..%d", kMaxExperts);
   const PlanShape s = plan_shape(M);
   return s.mode == kGrid ? static_cast<int64_t>(s.ctas) * (E + 1) * 4 : 0;
 }

@@ -162,20 +162,33 @@ __global__ void __launch_bounds__(kClipThreads) grad_norm_finish_kernel(const do
   if (threadIdx.x == 0) *norm = static_cast<float>(r);
 }
 
+// The factor as a product of two in the accumulator's type, the second a power of two and 1 unless the first
+// alone would be near the end of fp32's range: an element times a factor of 1e-50 need not be 0.
+template <typename A>
+struct Split {
+  A a, b;
+};
+template <typename A>
+__device__ __forceinline__ Split<A> split(double f) {
+  if (sizeof(A) == 8 || !(f > 0.0 && f < 0x1p-60)) return {static_cast<A>(f), A(1)};
+  const int m = min(126, -ilogb(f) / 2);  // both halves, and the product in between, stay in range
+  return {static_cast<A>(ldexp(f, m)), static_cast<A>(ldexp(1.0, -m))};
+}
+
 template <int U, typename T>
 __device__ void scale_chunk(const T* src, T* dst, int n, double c, int me, int threads, uint64_t policy) {
   using A = typename Acc<T>::type;
   constexpr int NV = 16 / sizeof(T);
-  const A f = static_cast<A>(c);
+  const Split<A> f = split<A>(c);
   const uintptr_t s = reinterpret_cast<uintptr_t>(src), d = reinterpret_cast<uintptr_t>(dst);
   if ((s ^ d) & 15) {  // no vector of one is a vector of the other
-    for (int i = me; i < n; i += threads) dst[i] = from_acc<T>(to_acc<T>(src[i]) * f);
+    for (int i = me; i < n; i += threads) dst[i] = from_acc<T>(to_acc<T>(src[i]) * f.a * f.b);
     return;
   }
   const int head = min(n, static_cast<int>((16 - (s & 15)) & 15) / static_cast<int>(sizeof(T)));
   const int nvec = (n - head) / NV, tail = head + nvec * NV;
-  for (int i = me; i < head; i += threads) dst[i] = from_acc<T>(to_acc<T>(src[i]) * f);
-  for (int i = tail + me; i < n; i += threads) dst[i] = from_acc<T>(to_acc<T>(src[i]) * f);
+  for (int i = me; i < head; i += threads) dst[i] = from_acc<T>(to_acc<T>(src[i]) * f.a * f.b);
+  for (int i = tail + me; i < n; i += threads) dst[i] = from_acc<T>(to_acc<T>(src[i]) * f.a * f.b);
   for (int v = me; v < nvec; v += threads * U) {
     Raw<16> r[U];
 #pragma unroll
@@ -190,7 +203,7 @@ __device__ void scale_chunk(const T* src, T* dst, int n, double c, int me, int t
         A x[NV];
         expand<T, 16>(r[u], x);
 #pragma unroll
-        for (int j = 0; j < NV; ++j) x[j] *= f;
+        for (int j = 0; j < NV; ++j) x[j] = x[j] * f.a * f.b;
         st_row_hint<16>(dst + head + static_cast<int64_t>(i) * NV, narrow<T, 16>(x), policy);
       }
     }

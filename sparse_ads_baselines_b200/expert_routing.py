@@ -29,7 +29,8 @@ MAX_CHOICES = 32
 
 class ExpertPlan(NamedTuple):
     """Where every choice goes: ``offsets`` int32 ``[E+1]`` (rows of every expert), ``positions`` int32
-    ``[N, k]`` (row of every choice) and ``order`` int32 ``[N*k]`` (the choice ``t*k + s`` in every row)."""
+    ``[N, k]`` (row of every choice) and ``order`` int32 ``[N*k]`` (the choice ``t*k + s`` in every row).
+    :func:`plan` makes one; a plan of your own needs ``positions`` to be a permutation of ``0 .. N*k-1``."""
     offsets: torch.Tensor
     positions: torch.Tensor
     order: torch.Tensor

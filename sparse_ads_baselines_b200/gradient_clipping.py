@@ -31,7 +31,8 @@ def _as_list(tensors):
 
 def grad_norm(tensors):
     """The 2-norm over all elements of ``tensors`` (a tensor or an iterable; None entries are left out), a
-    float32 scalar on their device.  Sums are kept in float64.  An empty list has norm 0."""
+    float32 scalar on their device (inf where it passes float32's range).  Sums are kept in float64.  An
+    empty list has norm 0."""
     return _lib.glue().grad_norm(_as_list(tensors))
 
 
@@ -39,8 +40,8 @@ def clip_grad_norm(tensors, max_norm, eps=1e-6, out=None):
     """Scales ``tensors`` by ``min(1, max_norm / (norm + eps))`` and returns ``norm``, the 2-norm over all of
     them as they came in (see :func:`grad_norm`).
 
-    In place, or, with ``out`` (as many tensors, of the same shapes, strides and types), into ``out``.  Every
-    element is rounded once.  A norm of NaN makes every element NaN and an infinite one every finite element
+    In place, or, with ``out`` (as many tensors, of the same shapes, strides and types), into ``out``.  The
+    factor is taken in float64 and every element is rounded once.  A norm of NaN makes every element NaN and an infinite one every finite element
     0, as the formula says: nothing is checked on the host.  A list in which two tensors share memory is
     refused, since an element must not be scaled twice."""
     if out is not None:

@@ -35,7 +35,8 @@ def _make(sizes, dtype, device, seed=0, scale=1.0):
 def _check(before, after, norm, max_norm, eps=1e-6):
     n = _norm(before)
     assert norm.dtype == torch.float32 and norm.dim() == 0
-    assert abs(float(norm) - n) <= NORM_TOL * n + 2.0 ** -150
+    # the returned float32 is inf where the norm passes its range (2^128, less a rounding); the factor is not
+    assert math.isinf(float(norm)) if n >= 2.0 ** 128 else abs(float(norm) - n) <= NORM_TOL * n + 2.0 ** -150
     c = min(1.0, max_norm / (n + eps))
     for b, a in zip(before, after):
         d = name(a.dtype)
@@ -134,6 +135,11 @@ def test_range(cuda_device, dtype):
         n = _norm(before)
         g = [t.clone() for t in before]
         _check(before, g, gc.clip_grad_norm(g, n / 3, eps=0.0), n / 3, eps=0.0)
+    if dtype != torch.float16:  # a factor below float32's range, elements that are not
+        for high, low in ((1e30, 1e-20), (1e20, 1e-24), (1e36, 1e-10)):
+            before = _make([1000, 300_000], dtype, cuda_device, scale=high)
+            g = [t.clone() for t in before]
+            _check(before, g, gc.clip_grad_norm(g, low, eps=0.0), low, eps=0.0)
     zero = [torch.zeros(5000, dtype=dtype, device=cuda_device)]
     assert float(gc.clip_grad_norm(zero, 1.0)) == 0.0 and not zero[0].any()
 

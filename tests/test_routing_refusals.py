@@ -50,10 +50,12 @@ def test_bad_arguments_of_the_c_entries(lib):
     refused(lib.tbe_expert_plan_workspace_bytes(-1, 4), b"M must be")
     refused(lib.tbe_expert_plan_workspace_bytes(1 << 31, 4), b"M must be")
     refused(lib.tbe_expert_plan_workspace_bytes(8, 0), b"E 1..1024")
-    assert lib.tbe_expert_plan_workspace_bytes(8192, 1024) == 0
-    need = lib.tbe_expert_plan_workspace_bytes(100_000, 1024)
+    refused(lib.tbe_expert_plan_workspace_bytes((1 << 31) - 1024, 4), b"M must be")
+    assert lib.tbe_expert_plan_workspace_bytes((1 << 31) - 1025, 4) > 0
+    assert lib.tbe_expert_plan_workspace_bytes(131_072, 1024) == 0
+    need = lib.tbe_expert_plan_workspace_bytes(200_000, 1024)
     assert need > 0
-    refused(lib.tbe_expert_plan(p, p, p, p, 100_000, 1024, p, need - 1, None), b"workspace")
+    refused(lib.tbe_expert_plan(p, p, p, p, 200_000, 1024, p, need - 1, None), b"workspace")
     refused(lib.tbe_expert_plan(p, None, p, p, 8, 4, None, 0, None), b"null")
     refused(lib.tbe_expert_dispatch(None, 4, p, p, p, 1, 1, 4, 2, f32, None), b"null")
     refused(lib.tbe_expert_dispatch(p, 4, p, p, p, 1, 0, 4, 2, f32, None), b"k and D > 0")
