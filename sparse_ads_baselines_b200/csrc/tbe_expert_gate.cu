@@ -26,6 +26,7 @@ namespace tbe {
 namespace {
 
 constexpr int kGateThreads = 256;
+constexpr int64_t kManyRows = 16384;  // rows from which a warp takes several
 constexpr int kGateMaxExperts = 1024;
 constexpr int kGateMaxK = 32;
 
@@ -76,19 +77,16 @@ struct Key<__nv_bfloat16> : Key16<__nv_bfloat16> {
 template <>
 struct Key<float> {
   using type = unsigned long long;
+  __device__ static __forceinline__ type one(float v, int c) {
+    const uint32_t b = __float_as_uint(__fadd_rn(v, 0.f));  // as above
+    const uint32_t o = b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+    return (static_cast<type>(o) << 32) | static_cast<uint32_t>(0xffff - c);
+  }
   __device__ static __forceinline__ void of(const float* v, int c0, int c1, type* key) {
     key[0] = one(v[0], c0);
     key[1] = one(v[1], c1);
   }
-  __device__ static __forceinline__ bool alive(type k) { return k != 0; }
-  __device__ static __forceinline__ type one(float v, int c) {
-    if (v == -INFINITY) return 0ull;
-    uint32_t b = __float_as_uint(v);
-    if (b == 0x80000000u) b = 0;
-    uint32_t o = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-    if (isnan(v)) o = 0xffffffffu;
-    return (static_cast<type>(o) << 32) | static_cast<uint32_t>(0xffff - c);
-  }
+  __device__ static __forceinline__ bool alive(type k) { return static_cast<uint32_t>(k >> 32) > 0x007fffffu; }
   __device__ static __forceinline__ float value(type k) {
     const uint32_t o = static_cast<uint32_t>(k >> 32);
     return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
@@ -145,6 +143,17 @@ __device__ __forceinline__ unsigned __int128 group_max(unsigned __int128 v, int 
     v = o > v ? o : v;
   }
   return v;
+}
+
+template <typename K>
+__device__ __forceinline__ K shuffle(K v, int from) {
+  if constexpr (sizeof(K) == 16) {
+    const unsigned long long hi = __shfl_sync(kFullMask, static_cast<unsigned long long>(v >> 64), from);
+    const unsigned long long lo = __shfl_sync(kFullMask, static_cast<unsigned long long>(v), from);
+    return (static_cast<K>(hi) << 64) | lo;
+  } else {
+    return __shfl_sync(kFullMask, v, from);
+  }
 }
 
 // Eight keys, largest first (Batcher's odd-even merge network, 19 comparators).
@@ -317,10 +326,102 @@ __global__ void __launch_bounds__(kGateThreads) gate_kernel(GateArgs a) {
   }
 }
 
+// R rows per warp, one after the other, so that what comes after the choice -- exponentials, sums, divisions,
+// stores -- is done once for all of them: lane r * (32 / R) + s ends up with the s-th choice of the r-th row.
+// Needs k <= 32 / R and k V <= 128.
+template <typename T, int V, int VE, int R>
+__global__ void __launch_bounds__(kGateThreads) gate_rows_kernel(GateArgs a) {
+  using A = typename Acc<T>::type;
+  using K = typename Key<T>::type;
+  constexpr int W = 32 / R;
+  __shared__ __align__(16) K room[kGateThreads / 32][128];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, slot = lane % W;
+  const int64_t row0 = (static_cast<int64_t>(blockIdx.x) * (kGateThreads >> 5) + warp) * R;
+  T v[R][V];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    load_row<T, V, VE>(static_cast<const T*>(a.logits) + (row0 + r) * a.stride, row0 + r < a.N, a.E, lane, 5, v[r]);
+  K mine = 0;
+  A top = 0, sum = 0;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    K key[V];
+#pragma unroll
+    for (int i = 0; i < V; i += 2) Key<T>::of(v[r] + i, column<VE>(i, lane, 5), column<VE>(i + 1, lane, 5), key + i);
+    A row_top = 0, row_sum = 0;
+    auto first = [&](K m) {
+      row_top = Key<T>::alive(m) ? Key<T>::value(m) : A(0);
+      if (!a.renormalize) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) row_sum += exp(to_acc<T>(v[r][i]) - row_top);  // -inf adds 0
+#pragma unroll
+        for (int m2 = 1; m2 < 32; m2 <<= 1) row_sum += __shfl_xor_sync(kFullMask, row_sum, m2);
+      }
+    };
+    K got = a.k * V <= 64 ? take_from_best_lanes<V, 2>(key, a.k, lane, room[warp], first)
+                          : take_from_best_lanes<V, 4>(key, a.k, lane, room[warp], first);
+    __syncwarp();  // `room` is read; the next row may write it
+    got = shuffle(got, slot);
+    if (lane / W == r) {
+      mine = got;
+      top = row_top;
+      sum = row_sum;
+    }
+  }
+  const bool chosen = slot < a.k && Key<T>::alive(mine);
+  const A e = chosen ? exp(Key<T>::value(mine) - top) : A(0);
+  if (a.renormalize) {
+    sum = e;
+#pragma unroll
+    for (int m = 1; m < W; m <<= 1) sum += __shfl_xor_sync(kFullMask, sum, m);
+  }
+  const int64_t row = row0 + lane / W;
+  if (row < a.N && slot < a.k) {
+    const int64_t at = row * a.k + slot;
+    a.experts[at] = chosen ? Key<T>::col(mine) : -1;
+    static_cast<A*>(a.weights)[at] = chosen ? e / sum : A(0);
+  }
+}
+
+// The gradient of renormalized weights, which is zero but on the chosen columns: R rows per warp are filled
+// with zeros in wide stores and then, behind a barrier of the warp, written to by the lanes that hold the
+// slots.  (65536 rows of 256 bf16, k = 8: 13 us for assembling the rows in shared memory first.)
+template <typename T, int VE, int R>
+__global__ void __launch_bounds__(kGateThreads) gate_backward_chosen_kernel(GateArgs a) {
+  using A = typename Acc<T>::type;
+  constexpr int W = 32 / R;
+  const int lane = threadIdx.x & 31, slot = lane % W;
+  const int64_t row0 = (static_cast<int64_t>(blockIdx.x) * (kGateThreads >> 5) + (threadIdx.x >> 5)) * R;
+  const int64_t row = row0 + lane / W;
+  A w = 0, g = 0;
+  int col = -1;
+  if (row < a.N && slot < a.k) {
+    const int64_t at = row * a.k + slot;
+    col = a.experts[at];  // (three independent loads)
+    w = static_cast<const A*>(a.weights)[at];
+    g = static_cast<const A*>(a.grad_weights)[at];
+    if (col < 0 || col >= a.E) {
+      col = -1;
+      w = g = A(0);
+    }
+  }
+  T* out = static_cast<T*>(a.grad_logits);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (row0 + r >= a.N) break;
+    for (int c = lane * VE; c < a.E; c += 32 * VE) st_row<VE * sizeof(T)>(out + (row0 + r) * a.E + c, raw_none<VE * sizeof(T)>());
+  }
+  A c = w * g;
+#pragma unroll
+  for (int m = 1; m < W; m <<= 1) c += __shfl_xor_sync(kFullMask, c, m);
+  __syncwarp();
+  if (col >= 0) out[row * a.E + col] = from_acc<T>(w * (g - c));
+}
+
 // Gradient of the logits, with c = sum_s w_s g_s:
 //   renormalize: dl = w_s (g_s - c) on the chosen, 0 elsewhere;   otherwise: dl_j = p_j (g_j [chosen] - c).
-// The chosen columns' terms are put into a row of shared memory by the lane that holds the slot and read
-// back by the lane that owns the column.
+// This kernel is the second; gate_backward_chosen_kernel is the first.  The chosen columns' g are put into a
+// row of shared memory by the lane that holds the slot and read back by the lane that owns the column.
 template <typename T, int V, int VE>
 __global__ void __launch_bounds__(kGateThreads) gate_backward_kernel(GateArgs a) {
   using A = typename Acc<T>::type;
@@ -347,74 +448,90 @@ __global__ void __launch_bounds__(kGateThreads) gate_backward_kernel(GateArgs a)
   }
   const A c = group_sum(w * g, glog);
   __syncwarp();
-  if (col >= 0) term[col] = a.renormalize ? w * (g - c) : g;
+  if (col >= 0) term[col] = g;
   __syncwarp();
 
   T* out = static_cast<T*>(a.grad_logits) + row * a.E;
-  A p[V];
-  if (!a.renormalize) {
-    T v[V];
-    load_row<T, V, VE>(static_cast<const T*>(a.logits) + row * a.stride, live, a.E, sub, glog, v);
-    A top = -INFINITY;
-    bool nan = false;
+  T v[V];
+  load_row<T, V, VE>(static_cast<const T*>(a.logits) + row * a.stride, live, a.E, sub, glog, v);
+  A p[V], top = -INFINITY;
+  bool nan = false;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      p[i] = to_acc<T>(v[i]);
-      top = p[i] > top ? p[i] : top;
-      nan |= isnan(p[i]);
-    }
-    for (int m = 1; m < (1 << glog); m <<= 1) {
-      const A o = __shfl_xor_sync(kFullMask, top, m);
-      top = o > top ? o : top;
-    }
-    const bool none = top == -INFINITY;
-    A sum = nan ? A(NAN) : A(0);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      p[i] = p[i] == -INFINITY ? A(0) : exp(p[i] - top);
-      sum += p[i];
-    }
-    sum = group_sum(sum, glog);
-#pragma unroll
-    for (int i = 0; i < V; ++i) p[i] = none && !isnan(sum) ? A(0) : p[i] / sum;
+  for (int i = 0; i < V; ++i) {
+    p[i] = to_acc<T>(v[i]);
+    top = p[i] > top ? p[i] : top;
+    nan |= isnan(p[i]);
   }
+  for (int m = 1; m < (1 << glog); m <<= 1) {
+    const A o = __shfl_xor_sync(kFullMask, top, m);
+    top = o > top ? o : top;
+  }
+  const bool none = top == -INFINITY;
+  A sum = nan ? A(NAN) : A(0);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    p[i] = p[i] == -INFINITY ? A(0) : exp(p[i] - top);
+    sum += p[i];
+  }
+  sum = group_sum(sum, glog);
+#pragma unroll
+  for (int i = 0; i < V; ++i) p[i] = none && !isnan(sum) ? A(0) : p[i] / sum;
 #pragma unroll
   for (int i = 0; i < V; i += VE) {
     const int col0 = column<VE>(i, sub, glog);
     if (!live || col0 >= a.E) continue;
     A d[VE];
 #pragma unroll
-    for (int j = 0; j < VE; ++j) {
-      d[j] = term[col0 + j];
-      if (!a.renormalize) d[j] = p[i + j] * (d[j] - c);
-    }
+    for (int j = 0; j < VE; ++j) d[j] = p[i + j] * (term[col0 + j] - c);
     st_row<VE * sizeof(T)>(out + col0, narrow<T, VE * sizeof(T)>(d));
   }
 }
 
+int64_t blocks_for(int64_t rows, int64_t rows_per_block) { return (rows + rows_per_block - 1) / rows_per_block; }
+
 template <typename T, int V, int VE>
 int launch_gate(const GateArgs& a, bool backward, cudaStream_t stream) {
-  const int64_t rows_per_block = static_cast<int64_t>(kGateThreads >> a.glog);
-  const int64_t blocks = (a.N + rows_per_block - 1) / rows_per_block;
-  if (blocks > 0x7fffffff) return fail(TBE_ERR_INVALID_ARGUMENT, "tbe_expert_gate: too many rows");
+  const unsigned blocks = static_cast<unsigned>(blocks_for(a.N, kGateThreads >> a.glog));
   if (!backward) {
+    constexpr int R = V == 8 ? 4 : 2;
     KernelTimer timer("gate_kernel", stream);
-    if (a.glog == 5) gate_kernel<T, V, VE, true><<<static_cast<unsigned>(blocks), kGateThreads, 0, stream>>>(a);
-    else if constexpr (V == 8) gate_kernel<T, V, VE, false><<<static_cast<unsigned>(blocks), kGateThreads, 0, stream>>>(a);
+    bool many = false;
+    if constexpr (sizeof(T) == 2) {
+      many = a.glog == 5 && a.k * R <= 32 && a.k * V <= 128 && a.N >= kManyRows;
+      if (many)
+        gate_rows_kernel<T, V, VE, R>
+            <<<static_cast<unsigned>(blocks_for(a.N, (kGateThreads >> 5) * R)), kGateThreads, 0, stream>>>(a);
+    }
+    if (many) {
+    } else if (a.glog == 5) gate_kernel<T, V, VE, true><<<blocks, kGateThreads, 0, stream>>>(a);
+    else if constexpr (V == 8) gate_kernel<T, V, VE, false><<<blocks, kGateThreads, 0, stream>>>(a);
   } else {
     KernelTimer timer("gate_backward_kernel", stream);
     const size_t shared = sizeof(typename Acc<T>::type) * kGateThreads * V;  // at most 64 KB (fp64, V = 32)
     if (shared > 48 * 1024)
       TBE_CUDA_TRY(cudaFuncSetAttribute(gate_backward_kernel<T, V, VE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         static_cast<int>(shared)));
-    gate_backward_kernel<T, V, VE><<<static_cast<unsigned>(blocks), kGateThreads, shared, stream>>>(a);
+    gate_backward_kernel<T, V, VE><<<blocks, kGateThreads, shared, stream>>>(a);
   }
   TBE_CHECK_LAUNCH(backward ? "gate_backward_kernel" : "gate_kernel");
   return TBE_OK;
 }
 
+template <typename T, int VE, int R>
+int launch_backward_chosen(const GateArgs& a, cudaStream_t stream) {
+  {
+    KernelTimer timer("gate_backward_chosen_kernel", stream);
+    gate_backward_chosen_kernel<T, VE, R>
+        <<<static_cast<unsigned>(blocks_for(a.N, (kGateThreads >> 5) * R)), kGateThreads, 0, stream>>>(a);
+  }
+  TBE_CHECK_LAUNCH("gate_backward_chosen_kernel");
+  return TBE_OK;
+}
+
 template <typename T, int VE>
 int launch_gate_width(const GateArgs& a, bool backward, cudaStream_t stream) {
+  if (backward && a.renormalize)
+    return a.k <= 8 ? launch_backward_chosen<T, VE, 4>(a, stream) : launch_backward_chosen<T, VE, 1>(a, stream);
   const int per_lane = (a.E + (1 << a.glog) - 1) >> a.glog;
   if (per_lane <= 8) return launch_gate<T, 8, VE>(a, backward, stream);
   if (per_lane <= 16) return launch_gate<T, 16, VE>(a, backward, stream);
@@ -432,6 +549,7 @@ int launch_gate_type(const GateArgs& a, bool backward, cudaStream_t stream) {
 }
 
 int run_gate(const char* who, GateArgs a, int dtype, bool backward, cudaStream_t stream) {
+  TBE_REQUIRE(a.N < (1ll << 31), "%s: N must be below 2^31", who);
   TBE_REQUIRE(a.N >= 0 && a.E > 0 && a.E <= kGateMaxExperts, "%s: the number of experts must be 1..%d", who,
               kGateMaxExperts);
   TBE_REQUIRE(a.k > 0 && a.k <= a.E && a.k <= kGateMaxK, "%s: k must be 1..min(E, %d)", who, kGateMaxK);
