@@ -24,11 +24,14 @@ constexpr int kMaxExperts = 1024;
 constexpr int64_t kMaxEntries = 0x7fffffffll - 1024;  // 32-bit positions, and room for an index past the end
 namespace cg = cooperative_groups;
 
-// How many CTAs sort a plan, by its number of choices: one, one cluster (totals exchanged through
-// distributed shared memory), or a grid with a counting kernel in front (totals through global memory).
-constexpr int kPlanOne = 4096;
+// How many CTAs sort a plan, by its number of choices: one of 256 threads, one cluster of 1024-thread CTAs
+// (totals exchanged through distributed shared memory), or a grid with a counting kernel in front (totals
+// through global memory).  64 experts, us on the GPU (one / cluster / grid): 1024 choices 4.0 / 4.5 / 6.6,
+// 2048 5.5 / 4.6 / 7.7, 65536 - / 10.2 / 12.8, 131072 - / 15.8 / 13.3, and a launch costs the host 4 us.
+constexpr int kPlanOne = 1024;
 constexpr int kPlanCluster = 8;
 constexpr int kPlanClusterMost = 131072;
+constexpr int64_t kFewVectors = 148 * 512;  // a quarter of the threads the GPU holds
 constexpr int kPlanSlice = 8192;  // choices per CTA of the grid, at least
 enum PlanMode { kOne, kCluster, kGrid };
 
@@ -40,6 +43,7 @@ struct PlanArgs {
   int32_t* order;
   int32_t* counts;  // [ctas][E+1], two-kernel plan only
   int32_t M, E, slice;
+  int32_t bits;  // of E + 1, the bin of a lane without a choice
 };
 
 __device__ __forceinline__ int bin_of(int32_t id, int E) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(E) ? id : E; }
@@ -71,7 +75,8 @@ __device__ void block_exclusive_scan(int32_t* v, int n, int32_t* warp_sums) {
 
 // One CTA sorts its slice: every warp counts a contiguous part per bin, the parts are prefix-summed warp
 // by warp, and a second pass in the same order places each choice behind the earlier ones of its bin.
-// The order is therefore the stable one, whatever the atomics of the counting did.
+// The order is therefore the stable one, whatever the atomics of the counting did.  Bound by latency (loads,
+// barriers) and by what a warp issues per 32 choices, not by its 12 bytes per choice.
 //   shared: hist[warps][E+1], start[E+1], before[E+1], own[E+1], 32 words
 template <int MODE>
 __global__ void __launch_bounds__(1024) plan_place_kernel(PlanArgs a) {
@@ -153,7 +158,12 @@ __global__ void __launch_bounds__(1024) plan_place_kernel(PlanArgs a) {
     const bool on = i < we;
     const int b = on ? bin_of(ahead, a.E) : E1;
     if (i + 32 < we) ahead = __ldg(a.experts + i + 32);
-    const unsigned peers = __match_any_sync(kFullMask, b);
+    unsigned peers = kFullMask;  // the lanes of the same bin (32768 choices, 64 experts: 9.4 us with match.any, 7.4 so)
+    for (int bit = 0; bit < a.bits; ++bit) {
+      const bool set = (b >> bit) & 1;
+      const unsigned with = __ballot_sync(kFullMask, set);
+      peers &= set ? with : ~with;
+    }
     const int rank = __popc(peers & ((1u << lane) - 1));
     const int32_t first = on ? next[b] : 0;
     __syncwarp();
@@ -213,6 +223,8 @@ __device__ __forceinline__ uint32_t kept_rows(const int32_t* kept, int32_t M) {
 
 // A thread takes U vectors of one sample's row, a U-th of the row apart, so that a warp's loads stay
 // contiguous and the positions are looked up once for all of them: U independent loads, then k stores each.
+// 2048 rows of 8192 fp16, k = 2: 16 us for 101 MB (6.3 TB/s).  Rows that are only aligned to 4 bytes are
+// bound by the load-store unit: 5003 of 1001 fp32, k = 6: 29 us for 140 MB (4.8 TB/s).
 template <int VB, int U>
 __global__ void __launch_bounds__(256) dispatch_kernel(RowArgs a) {
   const uint32_t i = blockIdx.x * 256u + threadIdx.x;
@@ -239,7 +251,10 @@ __global__ void __launch_bounds__(256) dispatch_kernel(RowArgs a) {
   }
 }
 
-// The same U vectors, summed over the sample's rows; KB * U row loads are in flight together.
+// The same U vectors, summed over the sample's rows; KB * U row loads are in flight together, in 64 registers
+// (four CTAs per SM).  8192 rows of 2048 bf16, us for (KB, U) = (1, 4) / (2, 1) / (2, 2) / (4, 1) / (4, 2) / (8, 1):
+// k = 1 10.8 / 16.5 / 12.7 / 19.5 / 13.8 / 23.8, k = 2 15.9 / 18.9 / 15.5 / 22.4 / 16.6 / 25.7, k = 4 25.7 / 28.8 /
+// 24.5 / 26.6 / 23.4 / 30.2, k = 8 45.9 / 49.0 / 43.3 / 44.4 / 41.7 / 42.6 (302 MB: 7.2 TB/s with L2's help).
 template <typename T, int VB, int U, int KB>
 __global__ void __launch_bounds__(256, 4) combine_kernel(RowArgs a) {
   using A = typename Acc<T>::type;
@@ -308,7 +323,11 @@ struct GradArgs {
 };
 
 // G lanes per sample walk its row, U vectors at a time: the upstream row is held in registers while KB
-// expert rows are read against it (dot products) and KB scaled copies are stored.
+// expert rows are read against it (dot products) and KB scaled copies are stored.  One pass for both
+// gradients: 16384 rows of 2048 bf16, k = 8, read 604 MB and write 537 in 174 us (6.6 TB/s, the copy rate).
+// G by the vectors of a row (16 M bf16 elements, k = 4; us with 8 / 32 / 128 lanes): 16 vectors 28 / 40 / 91,
+// 32 56 / 54 / 103, 96 68 / 52 / 53, 128 63 / 52 / 49.  KB by k (8192 x 2048 bf16; us with 2 / 4 / 8):
+// k = 2 28.6 / 29.2 / 38, 4 54 / 48 / 53, 8 105 / 95 / 89.
 template <typename T, int VB, int U, int G, int KB>
 __global__ void __launch_bounds__(G == 128 ? 128 : 256) combine_backward_kernel(GradArgs a) {
   using A = typename Acc<T>::type;
@@ -389,10 +408,8 @@ __global__ void __launch_bounds__(G == 128 ? 128 : 256) combine_backward_kernel(
 }
 
 // ---------------------------------------------------------------- launches
-// Vectors per thread: 16 bytes' worth, so that narrow vectors have as many loads in flight as wide ones.
 // (Combining 5003 rows of 1001 fp32 values, six choices each: 43 us with one 4-byte vector a thread, 34 with
 // two or four, 95 with eight.  dispatch has its k stores as well: 35 us with one, 29 with two, 30 with four.)
-constexpr int vectors_per_thread(int vb) { return vb == 16 ? 1 : vb == 8 ? 2 : 4; }
 
 // 32-bit thread indices: a launch covers as many samples as fit below 2^32 threads.  body(first sample,
 // arguments of the launch, blocks) launches one.
@@ -419,7 +436,7 @@ int per_sample_launches(const char* name, RowArgs a, int64_t N, int vb, int u, c
 
 template <int VB>
 int launch_dispatch(const RowArgs& a, int64_t N, cudaStream_t stream) {
-  constexpr int U = VB == 2 ? 4 : 2;
+  constexpr int U = VB == 2 ? 4 : 2;  // see above
   return per_sample_launches("dispatch_kernel", a, N, VB, U, stream, [&](int64_t n0, RowArgs b, unsigned blocks) {
     b.x = a.x + n0 * a.x_stride;
     dispatch_kernel<VB, U><<<blocks, 256, 0, stream>>>(b);
@@ -429,7 +446,7 @@ int launch_dispatch(const RowArgs& a, int64_t N, cudaStream_t stream) {
 template <typename T, int VB, int KB>
 int launch_combine_k(const RowArgs& a, int64_t N, cudaStream_t stream) {
   using A = typename Acc<T>::type;
-  constexpr int U = vectors_per_thread(VB) * (KB == 2 ? 2 : 1);  // at least four 16-byte loads in flight
+  constexpr int U = KB == 8 ? 1 : KB == 1 || VB < 8 ? 4 : 2;
   return per_sample_launches("combine_kernel", a, N, VB, U, stream, [&](int64_t n0, RowArgs b, unsigned blocks) {
     b.weights = a.weights ? static_cast<const A*>(a.weights) + n0 * a.k : nullptr;
     b.out = a.out + n0 * a.row_bytes;
@@ -442,9 +459,12 @@ int launch_combine(const RowArgs& a, int64_t N, cudaStream_t stream) {
   if constexpr (VB < static_cast<int>(sizeof(T))) {
     return fail(TBE_ERR_INVALID_ARGUMENT, "tbe_expert_combine: rows must be aligned to their element size");
   } else {
-    if (a.k <= 2) return launch_combine_k<T, VB, 2>(a, N, stream);
-    if (a.k <= 4) return launch_combine_k<T, VB, 4>(a, N, stream);
-    return launch_combine_k<T, VB, 8>(a, N, stream);
+    // a call too small to fill the GPU waits for its loads: all of a sample's at once (8 rows of 2048 bf16,
+    // k = 8: 2.3 us against 3.4)
+    if (a.k > 4 && N * (a.row_bytes / VB) <= kFewVectors) return launch_combine_k<T, VB, 8>(a, N, stream);
+    if (a.k == 1) return launch_combine_k<T, VB, 1>(a, N, stream);
+    if (a.k == 2) return launch_combine_k<T, VB, 2>(a, N, stream);
+    return launch_combine_k<T, VB, 4>(a, N, stream);
   }
 }
 
@@ -464,7 +484,7 @@ int launch_backward_gk(const GradArgs& a, cudaStream_t stream) {
   const int64_t blocks = (a.N + kThreads / G - 1) / (kThreads / G);
   {
     KernelTimer timer("combine_backward_kernel", stream);
-    combine_backward_kernel<T, VB, vectors_per_thread(VB), G, KB><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(a);
+    combine_backward_kernel<T, VB, VB == 16 ? 1 : VB == 8 ? 2 : 4, G, KB><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(a);
   }
   TBE_CHECK_LAUNCH("combine_backward_kernel");
   return TBE_OK;
@@ -529,9 +549,11 @@ extern "C" int tbe_expert_plan(const int32_t* experts, int32_t* offsets, int32_t
                 static_cast<long long>(workspace_bytes), static_cast<long long>(need));
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   const PlanShape s = plan_shape(M);
+  int bits = 1;
+  while (((E + 1) >> bits) != 0) ++bits;
   PlanArgs a{experts, offsets, positions, order, static_cast<int32_t*>(workspace), static_cast<int32_t>(M),
-             static_cast<int32_t>(E), s.slice};
-  const int threads = M <= 1024 ? 256 : 1024;
+             static_cast<int32_t>(E), s.slice, bits};
+  const int threads = s.mode == kOne ? 256 : 1024;
   const size_t shared = (static_cast<size_t>(threads / 32 + 3) * (E + 1) + 32) * 4;  // at most 144 KB
   auto place = s.mode == kOne ? plan_place_kernel<kOne> : s.mode == kCluster ? plan_place_kernel<kCluster> : plan_place_kernel<kGrid>;
   if (shared > 48 * 1024)

@@ -11,6 +11,8 @@
 // Bound by HBM.  The norm has to be known before the first element is scaled, so a list larger than L2 is
 // read twice; the scaling pass runs through the chunks backwards, so that what the norm pass read last is
 // still in L2.  In place and with c == 1 there is nothing to store and the second pass ends at once.
+// 200 M bf16 elements: 68 us for the norm (400 MB, 5.9 TB/s) and 123 us for the scaling (800 MB, 6.5 TB/s);
+// 300 M fp32 elements below the limit: 175 us (1.2 GB, 6.9 TB/s) and 3.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -29,7 +31,7 @@ constexpr int kClipBlocksPerSM = 8;   // norm pass (32 registers)
 constexpr int kScaleBlocksPerSM = 3;  // scaling pass (80): all resident, or the sweep would not run backwards
 constexpr int kChunk = 16384;      // elements
 constexpr int kSmallChunk = 1024;  // elements per warp of the one-kernel form
-constexpr int kSmallMost = 1 << 18;
+constexpr int kSmallMost = 1 << 17;  // elements; see grad_clip_small_kernel
 constexpr int kSmallCluster = 8;
 constexpr int kSmallTable = 64;    // tensors whose table fits a small parameter block
 constexpr int kLargeTable = 1024;  // and the largest (30 KB of parameters)
@@ -253,7 +255,9 @@ struct Owners {
 };
 
 // A short list in one launch: a cluster of CTAs, a warp per kSmallChunk elements, the CTAs' sums exchanged
-// through distributed shared memory between the two passes.
+// through distributed shared memory between the two passes.  The second launch of the two-kernel form costs
+// the host 4 us and the GPU a gap of about 1.5; on the GPU itself (one kernel / the two without the gap) 40 fp32
+// tensors of 1000 elements in all take 5.0 / 5.7 us, of 65536 7.5 / 5.8, of 131072 7.2 / 5.7, of 262144 11.0 / 6.7.
 template <int CAP>
 __global__ void __launch_bounds__(1024) grad_clip_small_kernel(const __grid_constant__ Table<CAP> t,
                                                                const __grid_constant__ Owners<CAP> owners, bool scale,

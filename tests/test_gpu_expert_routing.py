@@ -143,7 +143,7 @@ def test_gate_gradcheck(cuda_device):
 
 # ---------------------------------------------------------------------------- plan
 
-@pytest.mark.parametrize("N,k", [(0, 3), (1, 1), (1, 8), (7, 1), (128, 8), (129, 8), (512, 8), (4097, 1), (1025, 8),
+@pytest.mark.parametrize("N,k", [(0, 3), (1, 1), (1, 8), (7, 1), (128, 8), (129, 8), (1025, 1), (512, 8), (4097, 1), (1025, 8),
                                  (2731, 3), (20000, 2), (16384, 8), (131073, 1), (50001, 7), (200000, 8)])
 @pytest.mark.parametrize("E", [1, 2, 61, 256, 1024])
 def test_plan(cuda_device, N, k, E):

@@ -80,8 +80,9 @@ def test_many_tensors_of_mixed_types(cuda_device, count):
     assert abs(float(gc.grad_norm(mixed)) - _norm([t for t in mixed if t is not None])) <= NORM_TOL * float(norm)
 
 
-@pytest.mark.parametrize("sizes", [[2 ** 18], [2 ** 18 + 1], [2 ** 18 - 64] + [1] * 64, [255] * 1000, [2000] * 130,
-                                   [10 ** 6] + [3] * 70], ids=["one", "one more", "65", "1000", "130", "71"])
+@pytest.mark.parametrize("sizes", [[2 ** 17], [2 ** 17 + 1], [2 ** 17 - 64] + [1] * 64, [127] * 1000, [255] * 1000,
+                                   [2000] * 130, [10 ** 6] + [3] * 70],
+                         ids=["one", "one more", "65", "1000 short", "1000", "130", "71"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=name)
 def test_around_the_one_kernel_limit(cuda_device, sizes, dtype):
     before = _make(sizes, dtype, cuda_device)
