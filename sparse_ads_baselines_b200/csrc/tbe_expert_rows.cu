@@ -325,9 +325,10 @@ struct GradArgs {
 // G lanes per sample walk its row, U vectors at a time: the upstream row is held in registers while KB
 // expert rows are read against it (dot products) and KB scaled copies are stored.  One pass for both
 // gradients: 16384 rows of 2048 bf16, k = 8, read 604 MB and write 537 in 174 us (6.6 TB/s, the copy rate).
-// G by the vectors of a row (16 M bf16 elements, k = 4; us with 8 / 32 / 128 lanes): 16 vectors 28 / 40 / 91,
-// 32 56 / 54 / 103, 96 68 / 52 / 53, 128 63 / 52 / 49.  KB by k (8192 x 2048 bf16; us with 2 / 4 / 8):
-// k = 2 28.6 / 29.2 / 38, 4 54 / 48 / 53, 8 105 / 95 / 89.
+// G by the steps of a row, vectors / U (16 M bf16 elements in 16-byte vectors, k = 4; us with 8 / 32 / 128 lanes):
+// 16 steps 28 / 40 / 91, 32 56 / 54 / 103, 96 68 / 52 / 53, 128 63 / 52 / 49.  KB by k (8192 x 2048 bf16; us with
+// 2 / 4 / 8): k = 2 28.6 / 29.2 / 38, 4 54 / 48 / 53, 8 105 / 95 / 89; with vectors of 4 and 2 bytes, U = 4, eight
+// rows would take 128 registers and more (4096 x 2047 bf16, k = 8: 80 us with 4, 106 with 8).
 template <typename T, int VB, int U, int G, int KB>
 __global__ void __launch_bounds__(G == 128 ? 128 : 256) combine_backward_kernel(GradArgs a) {
   using A = typename Acc<T>::type;
@@ -478,13 +479,15 @@ int launch_combine_type(const RowArgs& a, int vb, int64_t N, cudaStream_t stream
   }
 }
 
+constexpr int backward_vectors(int vb) { return vb == 16 ? 1 : vb == 8 ? 2 : 4; }
+
 template <typename T, int VB, int G, int KB>
 int launch_backward_gk(const GradArgs& a, cudaStream_t stream) {
   constexpr int kThreads = G == 128 ? 128 : 256;
   const int64_t blocks = (a.N + kThreads / G - 1) / (kThreads / G);
   {
     KernelTimer timer("combine_backward_kernel", stream);
-    combine_backward_kernel<T, VB, VB == 16 ? 1 : VB == 8 ? 2 : 4, G, KB><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(a);
+    combine_backward_kernel<T, VB, backward_vectors(VB), G, KB><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(a);
   }
   TBE_CHECK_LAUNCH("combine_backward_kernel");
   return TBE_OK;
@@ -493,7 +496,7 @@ int launch_backward_gk(const GradArgs& a, cudaStream_t stream) {
 template <typename T, int VB, int G>
 int launch_backward_g(const GradArgs& a, cudaStream_t stream) {
   if (a.k <= 2) return launch_backward_gk<T, VB, G, 2>(a, stream);
-  if (a.k <= 4) return launch_backward_gk<T, VB, G, 4>(a, stream);
+  if (a.k <= 4 || VB < 8) return launch_backward_gk<T, VB, G, 4>(a, stream);
   return launch_backward_gk<T, VB, G, 8>(a, stream);
 }
 
@@ -503,8 +506,9 @@ int launch_backward(GradArgs a, cudaStream_t stream) {
     return fail(TBE_ERR_INVALID_ARGUMENT, "tbe_expert_combine_backward: rows must be aligned to their element size");
   } else {
     a.nvec = static_cast<int>(a.row_bytes / VB);
-    if (a.nvec <= 16) return launch_backward_g<T, VB, 8>(a, stream);
-    if (a.nvec <= 96) return launch_backward_g<T, VB, 32>(a, stream);
+    const int steps = (a.nvec + backward_vectors(VB) - 1) / backward_vectors(VB);
+    if (steps <= 16) return launch_backward_g<T, VB, 8>(a, stream);
+    if (steps <= 96) return launch_backward_g<T, VB, 32>(a, stream);
     return launch_backward_g<T, VB, 128>(a, stream);
   }
 }
