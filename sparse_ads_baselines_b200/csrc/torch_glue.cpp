@@ -357,11 +357,12 @@ Tensor clip_grad_norm(const std::vector<std::optional<Tensor>>& tensors, double 
   const c10::cuda::CUDAGuard guard(list.first->device());
   Tensor norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(list.first->device()));
   Tensor ws = norm_workspace(list);
+  // autograd notices that a saved tensor is written to (an inference tensor outside inference mode is refused here)
+  for (size_t i = 0; i < tensors.size(); ++i)
+    if (tensors[i].has_value()) (out ? *(*out)[i] : *tensors[i]).unsafeGetTensorImpl()->bump_version();
   must("tbe_grad_clip", tbe_grad_clip(list.address.data(), to.data(), list.size.data(), list.dtype.data(), list.count(),
                                       max_norm, eps, norm.data_ptr<float>(), ws.data_ptr(), ws.numel() * 8,
                                       stream_of(norm)));
-  for (const auto& t : out ? *out : tensors)  // autograd notices that a saved tensor was written to
-    if (t.has_value() && t->defined()) t->unsafeGetTensorImpl()->bump_version();
   return norm;
 }
 

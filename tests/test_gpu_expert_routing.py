@@ -84,6 +84,14 @@ def test_gate(cuda_device, N, E, k, dtype, renormalize, masked):
     assert torch.equal(w2, w) and torch.equal(e2, e)
 
 
+@pytest.mark.parametrize("N,E,k", [(16384, 256, 8), (16387, 130, 5), (16385, 512, 8), (16386, 999, 4), (16391, 256, 32),
+                                   (16384, 256, 9)])
+@pytest.mark.parametrize("dtype,renormalize,masked", [(torch.bfloat16, True, True), (torch.float16, False, False)],
+                         ids=["bfloat16-masked", "float16-whole"])
+def test_gate_many_rows(cuda_device, N, E, k, dtype, renormalize, masked):
+    test_gate(cuda_device, N, E, k, dtype, renormalize, masked)
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=name)
 def test_gate_strides(cuda_device, dtype):
     rng = np.random.default_rng(3)
@@ -444,6 +452,47 @@ def test_captured_training_step(cuda_device):
         torch.cuda.synchronize(cuda_device)
         want = step(logits.detach().clone().requires_grad_(), x.detach().clone().requires_grad_())
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("M", [100, 5000, 200_000])
+def test_captured_plan_of_many_experts(cuda_device, M):
+    """More shared memory than a kernel has without asking, in every form of the plan, captured and replayed."""
+    ids = torch.randint(0, 1024, (M, 1), dtype=torch.int32, device=cuda_device)
+    er.plan(ids, 1024)
+    torch.cuda.synchronize(cuda_device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = er.plan(ids, 1024)
+    for _ in range(2):
+        ids.copy_(torch.randint(-1, 1025, (M, 1), dtype=torch.int32, device=cuda_device))
+        graph.replay()
+        want = ref.plan(ids.cpu().numpy(), 1024)
+        assert all(np.array_equal(a.cpu().numpy(), b) for a, b in zip(got, want))
+
+
+def test_broadcast_inputs(cuda_device):
+    """One row or one weight for all samples: the gradient is summed over what was broadcast."""
+    rng, p, positions, kept = _cases(30, 2, 4, 24, torch.float64, 0.2, cuda_device)
+    row = _randn(rng, (24,), torch.float64, cuda_device).requires_grad_()
+    weight = _randn(rng, (2,), torch.float64, cuda_device).requires_grad_()
+    y = er.dispatch(row.expand(30, 24), p)
+    out = er.combine(y, p, weight.expand(30, 2))
+    g = _randn(rng, (30, 24), torch.float64, cuda_device)
+    d_row, d_weight = torch.autograd.grad(out, (row, weight), g)
+    here = torch.from_numpy(positions < kept).to(cuda_device).double()
+    # out[t] = (here[t] . weight) row
+    torch.testing.assert_close(d_row, ((here @ weight.detach())[:, None] * g).sum(0), rtol=1e-12, atol=1e-12)
+    torch.testing.assert_close(d_weight, (here * (g @ row.detach())[:, None]).sum(0), rtol=1e-12, atol=1e-12)
+
+
+def test_saved_tensors_that_change_are_noticed(cuda_device):
+    _, p, _, _ = _cases(10, 2, 4, 8, torch.float32, 0.0, cuda_device)
+    y = torch.randn(20, 8, device=cuda_device, requires_grad=True) * 1.0
+    w = torch.rand(10, 2, device=cuda_device, requires_grad=True)
+    out = er.combine(y, p, w)
+    y.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
 
 
 def test_same_bits_every_time(cuda_device):

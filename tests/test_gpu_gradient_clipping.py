@@ -188,6 +188,22 @@ def test_refusals(cuda_device):
     assert abs(float(gc.grad_norm(a)) - 1.0) < 1e-5
 
 
+def test_writes_are_noticed(cuda_device):
+    """A tensor that autograd has saved must not be scaled behind its back."""
+    a = torch.ones(10, device=cuda_device, requires_grad=True)
+    g = torch.full((10,), 3.0, device=cuda_device)
+    loss = (a * g).sum()
+    gc.clip_grad_norm([g], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        t = torch.ones(10, device=cuda_device)
+        assert float(gc.clip_grad_norm(t, 1.0)) > 3.0
+    with pytest.raises(RuntimeError):
+        gc.clip_grad_norm(t, 0.1)
+    assert float(t[0]) > 0.3
+
+
 def test_stream_and_graphs(cuda_device):
     """On another stream; captured twice with the two graphs replayed together on new values."""
     sizes = [3_000_000, 17, 65_000]
