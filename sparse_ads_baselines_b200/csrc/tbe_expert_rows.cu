@@ -221,22 +221,35 @@ __device__ __forceinline__ uint32_t kept_rows(const int32_t* kept, int32_t M) {
   return static_cast<uint32_t>(n < 0 ? 0 : n > M ? M : n);
 }
 
-// A thread takes U vectors of one sample's row, a U-th of the row apart, so that a warp's loads stay
-// contiguous and the positions are looked up once for all of them: U independent loads, then k stores each.
+// The U vectors of a thread: first, and the distance between them.  In a row of at least 32 U vectors (TILED) a
+// warp takes 32 U neighbouring ones, so that the distance is known at compile time and all of a thread's accesses
+// to a row are one address and constants; in a shorter row they lie a U-th of it apart.
+template <int VB, int U, bool TILED>
+struct Vectors {
+  uint32_t first, apart;
+  __device__ __forceinline__ Vectors(uint32_t place, uint32_t per_row)
+      : first(TILED ? (place >> 5) * (32 * U) + (place & 31) : place), apart(TILED ? 32 : per_row) {}
+  __device__ __forceinline__ uint32_t at(int u) const { return first + u * apart; }
+  __device__ __forceinline__ int64_t offset(int u) const {
+    return TILED ? static_cast<int64_t>(first) * VB + u * 32 * VB : static_cast<int64_t>(at(u)) * VB;
+  }
+};
+
+// A thread takes U vectors of one sample's row, so that a warp's loads stay contiguous and the positions are
+// looked up once for all of them: U independent loads, then k stores each.
 // 2048 rows of 8192 fp16, k = 2: 16 us for 101 MB (6.3 TB/s).  Rows that are only aligned to 4 bytes are
-// bound by the load-store unit: 5003 of 1001 fp32, k = 6: 29 us for 140 MB (4.8 TB/s).
-template <int VB, int U>
+// bound by the load-store unit: 5003 of 1001 fp32, k = 6: 26 us for 140 MB (5.4 TB/s; 29 without TILED).
+template <int VB, int U, bool TILED>
 __global__ void __launch_bounds__(256) dispatch_kernel(RowArgs a) {
   const uint32_t i = blockIdx.x * 256u + threadIdx.x;
   if (i >= a.items) return;
-  const uint32_t t = fastdiv(i, a.div), v0 = i - t * a.per_row;
+  const uint32_t t = fastdiv(i, a.div), place = i - t * a.per_row;
+  const Vectors<VB, U, TILED> v(place, a.per_row);
   const char* src = a.x + t * a.x_stride;
   Raw<VB> r[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint32_t v = v0 + u * a.per_row;
-    if (v < a.nvec) r[u] = ld_stream<VB>(src + static_cast<int64_t>(v) * VB);
-  }
+  for (int u = 0; u < U; ++u)
+    if (v.at(u) < a.nvec) r[u] = ld_stream<VB>(src + v.offset(u));
   const uint32_t kept = kept_rows(a.kept, a.M), M = static_cast<uint32_t>(a.M);
   const int32_t* pos = a.positions + static_cast<int64_t>(t) * a.k;
   for (int s = 0; s < a.k; ++s) {
@@ -244,10 +257,8 @@ __global__ void __launch_bounds__(256) dispatch_kernel(RowArgs a) {
     if (p >= M) continue;
     char* dst = a.out + p * a.row_bytes;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t v = v0 + u * a.per_row;
-      if (v < a.nvec) st_row<VB>(dst + static_cast<int64_t>(v) * VB, p < kept ? r[u] : raw_none<VB>());
-    }
+    for (int u = 0; u < U; ++u)
+      if (v.at(u) < a.nvec) st_row<VB>(dst + v.offset(u), p < kept ? r[u] : raw_none<VB>());
   }
 }
 
@@ -255,13 +266,14 @@ __global__ void __launch_bounds__(256) dispatch_kernel(RowArgs a) {
 // (four CTAs per SM).  8192 rows of 2048 bf16, us for (KB, U) = (1, 4) / (2, 1) / (2, 2) / (4, 1) / (4, 2) / (8, 1):
 // k = 1 10.8 / 16.5 / 12.7 / 19.5 / 13.8 / 23.8, k = 2 15.9 / 18.9 / 15.5 / 22.4 / 16.6 / 25.7, k = 4 25.7 / 28.8 /
 // 24.5 / 26.6 / 23.4 / 30.2, k = 8 45.9 / 49.0 / 43.3 / 44.4 / 41.7 / 42.6 (302 MB: 7.2 TB/s with L2's help).
-template <typename T, int VB, int U, int KB>
+template <typename T, int VB, int U, int KB, bool TILED>
 __global__ void __launch_bounds__(256, 4) combine_kernel(RowArgs a) {
   using A = typename Acc<T>::type;
   constexpr int NE = VB / sizeof(T);
   const uint32_t i = blockIdx.x * 256u + threadIdx.x;
   if (i >= a.items) return;
-  const uint32_t t = fastdiv(i, a.div), v0 = i - t * a.per_row;
+  const uint32_t t = fastdiv(i, a.div), place = i - t * a.per_row;
+  const Vectors<VB, U, TILED> v(place, a.per_row);
   const int64_t at = static_cast<int64_t>(t) * a.k;
   const uint32_t kept = kept_rows(a.kept, a.M);
   A acc[U][NE];
@@ -281,10 +293,8 @@ __global__ void __launch_bounds__(256, 4) combine_kernel(RowArgs a) {
       w[s] = in[s] && a.weights ? __ldg(static_cast<const A*>(a.weights) + at + s0 + s) : A(1);
       const char* src = a.x + p * a.x_stride;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint32_t v = v0 + u * a.per_row;
-        if (in[s] && v < a.nvec) r[s][u] = ld_stream<VB>(src + static_cast<int64_t>(v) * VB);
-      }
+      for (int u = 0; u < U; ++u)
+        if (in[s] && v.at(u) < a.nvec) r[s][u] = ld_stream<VB>(src + v.offset(u));
     }
 #pragma unroll
     for (int s = 0; s < KB; ++s) {
@@ -300,10 +310,8 @@ __global__ void __launch_bounds__(256, 4) combine_kernel(RowArgs a) {
   }
   char* dst = a.out + t * a.row_bytes;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint32_t v = v0 + u * a.per_row;
-    if (v < a.nvec) st_row<VB>(dst + static_cast<int64_t>(v) * VB, narrow<T, VB>(acc[u]));
-  }
+  for (int u = 0; u < U; ++u)
+    if (v.at(u) < a.nvec) st_row<VB>(dst + v.offset(u), narrow<T, VB>(acc[u]));
 }
 
 struct GradArgs {
@@ -417,7 +425,7 @@ __global__ void __launch_bounds__(G == 128 ? 128 : 256) combine_backward_kernel(
 template <typename F>
 int per_sample_launches(const char* name, RowArgs a, int64_t N, int vb, int u, cudaStream_t stream, F body) {
   a.nvec = static_cast<uint32_t>(a.row_bytes / vb);
-  a.per_row = (a.nvec + u - 1) / u;
+  a.per_row = a.nvec >= 32u * u ? (a.nvec + 32 * u - 1) / (32 * u) * 32 : (a.nvec + u - 1) / u;
   a.div = make_fastdiv(a.per_row);
   const int64_t knob = tuning(kTuneRowThreads), most = knob > 0 ? knob : 0xffffffffll - 4096;
   const int64_t step = most > a.per_row ? most / a.per_row : 1;  // per_row <= 2^28
@@ -440,7 +448,7 @@ int launch_dispatch(const RowArgs& a, int64_t N, cudaStream_t stream) {
   constexpr int U = VB == 2 ? 4 : 2;  // see above
   return per_sample_launches("dispatch_kernel", a, N, VB, U, stream, [&](int64_t n0, RowArgs b, unsigned blocks) {
     b.x = a.x + n0 * a.x_stride;
-    dispatch_kernel<VB, U><<<blocks, 256, 0, stream>>>(b);
+    (b.nvec >= 32u * U ? dispatch_kernel<VB, U, true> : dispatch_kernel<VB, U, false>)<<<blocks, 256, 0, stream>>>(b);
   });
 }
 
@@ -451,7 +459,8 @@ int launch_combine_k(const RowArgs& a, int64_t N, cudaStream_t stream) {
   return per_sample_launches("combine_kernel", a, N, VB, U, stream, [&](int64_t n0, RowArgs b, unsigned blocks) {
     b.weights = a.weights ? static_cast<const A*>(a.weights) + n0 * a.k : nullptr;
     b.out = a.out + n0 * a.row_bytes;
-    combine_kernel<T, VB, U, KB><<<blocks, 256, 0, stream>>>(b);
+    (b.nvec >= 32u * U ? combine_kernel<T, VB, U, KB, true>
+                       : combine_kernel<T, VB, U, KB, false>)<<<blocks, 256, 0, stream>>>(b);
   });
 }
 

@@ -97,7 +97,7 @@ variable_list once(variable_list grads) {
 // ---------------------------------------------------------------- gate
 std::tuple<Tensor, Tensor> gate_forward(const Tensor& logits, int64_t k, bool renormalize) {
   const c10::cuda::CUDAGuard guard(logits.device());
-  const Tensor rows = dense_rows(logits.detach());
+  const Tensor rows = dense_rows(logits);
   const int64_t N = rows.size(0), E = rows.size(1);
   Tensor weights = at::empty({N, k}, rows.options().dtype(weights_type(rows)));
   Tensor experts = at::empty({N, k}, rows.options().dtype(at::kInt));
@@ -177,7 +177,7 @@ void check_plan(const Tensor& offsets, const Tensor& positions, const Tensor& ro
 // ---------------------------------------------------------------- dispatch and combine
 Tensor dispatch_rows(const Tensor& x, const Tensor& offsets, const Tensor& positions) {
   const c10::cuda::CUDAGuard guard(x.device());
-  const Tensor rows = dense_rows(x.detach());
+  const Tensor rows = dense_rows(x);
   const int64_t N = positions.size(0), k = positions.size(1), D = rows.size(1);
   Tensor y = at::empty({N * k, D}, rows.options());
   must("tbe_expert_dispatch", tbe_expert_dispatch(rows.data_ptr(), rows.stride(0), ints(positions), ints(offsets),
@@ -188,8 +188,8 @@ Tensor dispatch_rows(const Tensor& x, const Tensor& offsets, const Tensor& posit
 
 Tensor combine_rows(const Tensor& y, const Tensor& offsets, const Tensor& positions, const Tensor& weights) {
   const c10::cuda::CUDAGuard guard(y.device());
-  const Tensor rows = y.detach().contiguous();
-  const Tensor w = weights.defined() ? weights.detach().contiguous() : Tensor();
+  const Tensor rows = y.contiguous();
+  const Tensor w = weights.defined() ? weights.contiguous() : Tensor();
   const int64_t N = positions.size(0), k = positions.size(1), D = rows.size(1);
   Tensor out = at::empty({N, D}, rows.options());
   must("tbe_expert_combine", tbe_expert_combine(rows.data_ptr(), ints(positions), ints(offsets), data(w), out.data_ptr(),
