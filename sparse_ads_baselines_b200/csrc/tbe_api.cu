@@ -101,7 +101,7 @@ int64_t device_l2_bytes() {
 }
 }  // namespace tbe
 
-extern "C" int tbe_abi_version(void) { return 5; }
+extern "C" int tbe_abi_version(void) { return 6; }
 
 extern "C" const char* tbe_last_error_string(void) { return tbe::g_error; }
 

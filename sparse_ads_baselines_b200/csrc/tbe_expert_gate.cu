@@ -20,8 +20,8 @@
 // row's maximum and sum from the logits when it needs them.
 //
 // Bound by instruction issue (78 % of the slots), not by HBM.  65536 rows of 256 bf16 logits, k = 8, are
-// 33.5 MB (5 us) and take 25 us: 54 us with k rounds over all keys, 33 with sorted runs, 30 with the best
-// lanes first, 25 with four rows per warp.  fp32: 45 us.  One row: 2.4 us, an empty kernel's time.
+// 33.5 MB (5 us) and take 25 us: 33 us with rounds over the sorted runs of all keys, 30 with the best lanes
+// first, 25 with four rows per warp.  fp32: 45 us.  One row: 2.4 us, about an empty kernel's time.
 #include "tbe_elem.cuh"
 
 namespace tbe {

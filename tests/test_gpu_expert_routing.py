@@ -357,7 +357,7 @@ def test_past_32_bit_offsets(cuda_device):
 def test_several_launches(cuda_device):
     """Calls beyond 2^32 threads are cut by samples; the knob makes small ones take the same way."""
     from sparse_ads_baselines_b200 import _lib
-    for D, dtype in ((64, torch.bfloat16), (33, torch.float32)):
+    for D, dtype in ((64, torch.bfloat16), (33, torch.float32), (1001, torch.float32), (1024, torch.float16)):
         rng, p, _, _ = _cases(100, 3, 8, D, dtype, 0.2, cuda_device)
         x = _randn(rng, (100, D + 3), dtype, cuda_device)[:, 1:D + 1]
         y = _randn(rng, (300, D), dtype, cuda_device)
