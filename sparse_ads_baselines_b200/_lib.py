@@ -120,6 +120,7 @@ def glue():
     global _glue
     if _glue is None:
         lib()
+        import torch  # noqa: F401  (its libraries have to be loaded first)
         try:
             from . import _torch_glue
         except ImportError as e:
