@@ -389,7 +389,8 @@ __global__ void __launch_bounds__(kGateThreads) gate_rows_kernel(GateArgs a) {
 
 // The gradient of renormalized weights, which is zero but on the chosen columns: R rows per warp are filled
 // with zeros in wide stores and then, behind a barrier of the warp, written to by the lanes that hold the
-// slots.  65536 rows of 256 bf16, k = 8 (33.5 MB written, 5 us): 9 us, 13 us for assembling the rows in
+// slots.  The weights sum to 1, so g_s - c is taken as sum_j w_j (g_s - g_j), which keeps its digits when one
+// weight is nearly 1 and c nearly that slot's g.  65536 rows of 256 bf16, k = 8 (33.5 MB written, 5 us): 9 us, 13 us for assembling the rows in
 // shared memory first.
 template <typename T, int VE, int R>
 __global__ void __launch_bounds__(kGateThreads) gate_backward_chosen_kernel(GateArgs a) {
@@ -416,11 +417,13 @@ __global__ void __launch_bounds__(kGateThreads) gate_backward_chosen_kernel(Gate
     if (row0 + r >= a.N) break;
     for (int c = lane * VE; c < a.E; c += 32 * VE) st_row<VE * sizeof(T)>(out + (row0 + r) * a.E + c, raw_none<VE * sizeof(T)>());
   }
-  A c = w * g;
-#pragma unroll
-  for (int m = 1; m < W; m <<= 1) c += __shfl_xor_sync(kFullMask, c, m);
+  A d = 0;
+  for (int s = 0; s < a.k; ++s) {
+    const A ws = __shfl_sync(kFullMask, w, lane - slot + s), gs = __shfl_sync(kFullMask, g, lane - slot + s);
+    d += ws * (g - gs);
+  }
   __syncwarp();
-  if (col >= 0) out[row * a.E + col] = from_acc<T>(w * (g - c));
+  if (col >= 0) out[row * a.E + col] = from_acc<T>(w * d);
 }
 
 // Gradient of the logits, with c = sum_s w_s g_s:

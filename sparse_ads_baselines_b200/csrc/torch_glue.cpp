@@ -63,6 +63,7 @@ at::ScalarType weights_type(const Tensor& rows) { return rows.scalar_type() == a
 void check_cuda(const char* name, const Tensor& t) {
   REQUIRE(t.defined() && t.is_cuda() && t.layout() == at::kStrided, name,
           " must be a CUDA tensor (this library has no CPU path)");
+  REQUIRE(!t.is_neg(), name, " is a lazily negated view: call resolve_neg() on it");
 }
 void check_int32(const char* name, const Tensor& t) {
   check_cuda(name, t);
@@ -293,6 +294,7 @@ struct List {
       REQUIRE(t.defined() && t.is_cuda(), "tensors must be CUDA tensors (this library has no CPU path)");
       REQUIRE(t.layout() == at::kStrided && dtype_of(t) >= 0,
               "tensors must be dense float16, bfloat16, float32 or float64 tensors");
+      REQUIRE(!t.is_neg(), "tensors must not be lazily negated views");
       REQUIRE(t.numel() == 0 || t.is_non_overlapping_and_dense(),
               "tensors must fill their memory without gaps or repeats (got strides ", t.strides(), " for ", t.sizes(), ")");
       if (!first) first = &t;
@@ -346,7 +348,7 @@ Tensor clip_grad_norm(const std::vector<std::optional<Tensor>>& tensors, double 
     const Tensor& t = *tensors[i];
     if (out) {
       const auto& o = (*out)[i];
-      REQUIRE(o.has_value() && o->defined() && o->layout() == at::kStrided && o->device() == t.device() &&
+      REQUIRE(o.has_value() && o->defined() && o->layout() == at::kStrided && !o->is_neg() && o->device() == t.device() &&
                   o->scalar_type() == t.scalar_type() && o->sizes() == t.sizes() && same_order(*o, t),
               "out must match tensors in device, type, shape and strides");
       to.push_back(o->data_ptr());

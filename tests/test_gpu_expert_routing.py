@@ -142,6 +142,26 @@ def test_gate_lowest_values(cuda_device):
         assert_within(w, np.array([[1 / 6] * 6, [0.25] * 4 + [0.0] * 2]), 1e-6)
 
 
+def test_gate_gradient_of_a_settled_router(cuda_device):
+    """One weight nearly 1: the renormalized gradient keeps its relative accuracy (every term of w_s sum_j w_j
+    (g_s - g_j) has the errors of two weights, 360 u, and of its operations; the gradients differ by more than an
+    eighth of the larger, so their difference costs no more than 16 u)."""
+    rng = np.random.default_rng(8)
+    x = torch.zeros(500, 40, device=cuda_device)
+    x[:, 7] = torch.from_numpy(rng.uniform(8, 14, 500)).float().to(cuda_device)
+    x.requires_grad_()
+    w, e = er.gate(x, 2)
+    g = torch.from_numpy(np.stack([rng.uniform(1, 2, 500), rng.uniform(-2, -1, 500)], 1)).float().to(cuda_device)
+    dx, = torch.autograd.grad(w, x, g)
+    wr, exr = ref.gate(f64(x), 2, True)
+    # the reference in the same form: in float64 the other one would do as well
+    first = wr[:, 0] * wr[:, 1] * (f64(g)[:, 0] - f64(g)[:, 1])
+    want = np.zeros((500, 40))
+    want[np.arange(500), exr[:, 0]], want[np.arange(500), exr[:, 1]] = first, -first
+    assert float(w[:, 0].min()) > 0.999
+    assert_within(dx, want, 400 * unit(torch.float32) * np.abs(want))
+
+
 def test_gate_gradcheck(cuda_device):
     torch.manual_seed(0)
     x = torch.randn(6, 20, dtype=torch.float64, device=cuda_device, requires_grad=True)
@@ -543,6 +563,7 @@ def test_refusals(cuda_device):
         lambda: er.dispatch(torch.zeros(4, 0, device=cuda_device), p),
         lambda: er.combine(y[:-1], p, w), lambda: er.combine(y, p, w[:3]), lambda: er.combine(y, p, w.half()),
         lambda: er.combine(y, p, w.cpu()), lambda: er.combine(y, None, w),
+        lambda: er.dispatch(torch._neg_view(x), p), lambda: er.combine(y, p, torch._neg_view(w)),
     ]
     for i, call in enumerate(bad):
         with pytest.raises(RuntimeError):
