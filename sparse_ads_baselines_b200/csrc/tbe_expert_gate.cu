@@ -428,8 +428,11 @@ __global__ void __launch_bounds__(kGateThreads) gate_backward_chosen_kernel(Gate
 
 // Gradient of the logits, with c = sum_s w_s g_s:
 //   renormalize: dl = w_s (g_s - c) on the chosen, 0 elsewhere;   otherwise: dl_j = p_j (g_j [chosen] - c).
-// This kernel is the second; gate_backward_chosen_kernel is the first.  The chosen columns' g are put into a
-// row of shared memory by the lane that holds the slot and read back by the lane that owns the column.
+// This kernel is the second; gate_backward_chosen_kernel is the first.  A chosen column's g_s - c is taken as
+//   sum_j w_j (g_s - g_j) + r g_s,   r = the mass of the columns that were not chosen, summed from their own p,
+// which keeps its digits when one weight is nearly 1 and c nearly that slot's g.  The lanes that hold the slots
+// mark their columns in a row of shared memory, the lanes that own the columns sum r from the unmarked ones, and
+// the slots' factors go the same way.
 template <typename T, int V, int VE>
 __global__ void __launch_bounds__(kGateThreads) gate_backward_kernel(GateArgs a) {
   using A = typename Acc<T>::type;
@@ -456,7 +459,7 @@ __global__ void __launch_bounds__(kGateThreads) gate_backward_kernel(GateArgs a)
   }
   const A c = group_sum(w * g, glog);
   __syncwarp();
-  if (col >= 0) term[col] = g;
+  if (col >= 0) term[col] = A(1);
   __syncwarp();
 
   T* out = static_cast<T*>(a.grad_logits) + row * a.E;
@@ -484,13 +487,31 @@ __global__ void __launch_bounds__(kGateThreads) gate_backward_kernel(GateArgs a)
   sum = group_sum(sum, glog);
 #pragma unroll
   for (int i = 0; i < V; ++i) p[i] = none && !isnan(sum) ? A(0) : p[i] / sum;
+
+  uint32_t picked = 0;  // of this lane's columns
+  A rest = 0;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const bool marked = term[column<VE>(i, sub, glog)] != A(0);
+    picked |= static_cast<uint32_t>(marked) << i;
+    rest += marked ? A(0) : p[i];
+  }
+  rest = group_sum(rest, glog);
+  A diff = rest * g;
+  for (int s = 0; s < a.k; ++s) {
+    const A ws = __shfl_sync(kFullMask, w, lane - sub + s), gs = __shfl_sync(kFullMask, g, lane - sub + s);
+    diff += ws * (g - gs);
+  }
+  __syncwarp();  // the marks are read
+  if (col >= 0) term[col] = diff;
+  __syncwarp();
 #pragma unroll
   for (int i = 0; i < V; i += VE) {
     const int col0 = column<VE>(i, sub, glog);
     if (!live || col0 >= a.E) continue;
     A d[VE];
 #pragma unroll
-    for (int j = 0; j < VE; ++j) d[j] = p[i + j] * (term[col0 + j] - c);
+    for (int j = 0; j < VE; ++j) d[j] = p[i + j] * (((picked >> (i + j)) & 1u) ? term[col0 + j] : A(0) - c);
     st_row<VE * sizeof(T)>(out + col0, narrow<T, VE * sizeof(T)>(d));
   }
 }

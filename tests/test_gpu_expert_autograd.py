@@ -1,0 +1,37 @@
+"""Gradients of the routing operators where digits cancel.
+
+Tolerances count roundings (u = 2^-24), as in the tests of the operators themselves.
+"""
+import numpy as np
+import pytest
+import torch
+
+import routing_testlib as ref
+from routing_testlib import assert_within, f64, unit
+from sparse_ads_baselines_b200 import expert_routing as er
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("E", [2, 40, 256, 1000])
+@pytest.mark.parametrize("k", [1, 2])
+def test_whole_softmax_gradient_of_a_settled_router(cuda_device, E, k):
+    """One weight nearly 1 (all other logits 0): the gradient keeps its relative accuracy in every column.
+
+    A p_j carries 2 units (4 u) of exp (the differences are exact), 37 roundings of the sum and 4 u of its terms,
+    one division: 46 u; a sum of them 37 more: 83 u.  p_s (sum over the chosen of w_j (g_s - g_j) + r g_s): the two
+    terms have one sign, each carries at most 83 u and 2 operations; their sum 1, p_s and the product 47: 133 u.
+    p_j c: c = w_1 g_1 + w_2 g_2 with |w_2 g_2| < w_1 |g_1| / 1000: 50 u, p_j and the product 47: 97 u."""
+    rng = np.random.default_rng(E + k)
+    x = torch.zeros(300, E, device=cuda_device)
+    x[:, 1] = torch.from_numpy(rng.uniform(8, 20, 300)).float().to(cuda_device)
+    x[0, 1], x[1, 1] = 20.0, 18.0
+    x.requires_grad_()
+    w, e = er.gate(x, k, renormalize=False)
+    g = torch.from_numpy(np.stack([rng.uniform(1, 2, 300), rng.uniform(-2, -1, 300)], 1)[:, :k]).float().to(cuda_device)
+    dx, = torch.autograd.grad(w, x, g)
+    exact = f64(x).astype(np.longdouble)  # the formula loses digits too: 2^-53 / 2e-9 of the smallest value in float64
+    weights, experts = ref.gate(exact, k, False)
+    want = ref.gate_gradient(exact, weights, experts, f64(g), False)[0].astype(np.float64)
+    assert np.array_equal(e.cpu().numpy(), experts)
+    assert_within(dx, want, 133 * unit(torch.float32) * np.abs(want))
