@@ -81,6 +81,9 @@ void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.devi
 int32_t* ints(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
 void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// An upstream gradient as the kernels read it: they see memory, not the negative bit that autograd may have set.
+Tensor incoming(const Tensor& grad) { return grad.detach().resolve_neg(); }
+
 // What a backward returns when its own graph is recorded: differentiating it again raises.
 variable_list once(variable_list grads) {
   if (at::GradMode::is_enabled())
@@ -123,7 +126,7 @@ struct Gate : Function<Gate> {
     const auto saved = ctx->get_saved_variables();
     const Tensor weights = saved[0].detach(), experts = saved[1];
     const c10::cuda::CUDAGuard guard(weights.device());
-    const Tensor g = grads[0].detach().contiguous();
+    const Tensor g = incoming(grads[0]).contiguous();
     const int64_t N = weights.size(0), k = weights.size(1), E = ctx->saved_data["experts"].toInt();
     Tensor out = at::empty({N, E}, weights.options().dtype(static_cast<at::ScalarType>(ctx->saved_data["dtype"].toInt())));
     const bool renormalize = !saved[2].defined();
@@ -207,7 +210,7 @@ struct Dispatch : Function<Dispatch> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
-    return once({combine_rows(grads[0], saved[0], saved[1], Tensor()), Tensor(), Tensor()});
+    return once({combine_rows(incoming(grads[0]), saved[0], saved[1], Tensor()), Tensor(), Tensor()});
   }
 };
 
@@ -220,7 +223,7 @@ struct Sum : Function<Sum> {  // combine without weights
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
-    return once({dispatch_rows(grads[0], saved[0], saved[1]), Tensor(), Tensor()});
+    return once({dispatch_rows(incoming(grads[0]), saved[0], saved[1]), Tensor(), Tensor()});
   }
 };
 
@@ -238,7 +241,7 @@ struct Combine : Function<Combine> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &offsets = saved[2], &positions = saved[3];
     const c10::cuda::CUDAGuard guard(offsets.device());
-    const Tensor g = dense_rows(grads[0].detach()), weights = saved[1].detach().contiguous();
+    const Tensor g = dense_rows(incoming(grads[0])), weights = saved[1].detach().contiguous();
     const Tensor y = need_w ? saved[0].detach().contiguous() : Tensor();
     const int64_t N = positions.size(0), k = positions.size(1), D = g.size(1);
     Tensor grad_y = need_y ? at::empty({N * k, D}, g.options()) : Tensor();

@@ -35,3 +35,34 @@ def test_whole_softmax_gradient_of_a_settled_router(cuda_device, E, k):
     want = ref.gate_gradient(exact, weights, experts, f64(g), False)[0].astype(np.float64)
     assert np.array_equal(e.cpu().numpy(), experts)
     assert_within(dx, want, 133 * unit(torch.float32) * np.abs(want))
+
+
+def _graph(op, device):
+    """(output, inputs) of one operator with its graph."""
+    torch.manual_seed(3)
+    x = torch.randn(6, 8, device=device)
+    if op.startswith("gate"):
+        x.requires_grad_()
+        return er.gate(x, 3, renormalize=op == "gate")[0], (x,)
+    p = er.plan(er.gate(x, 3)[1], 7)
+    if op == "dispatch":
+        x.requires_grad_()
+        return er.dispatch(x, p), (x,)
+    y = torch.randn(18, 8, device=device, requires_grad=True)
+    if op == "sum":
+        return er.combine(y, p), (y,)
+    w = torch.rand(6, 3, device=device, requires_grad=True)
+    return er.combine(y, p, w), (y, w)
+
+
+OPS = ["gate", "gate_whole", "dispatch", "sum", "combine"]
+
+
+@pytest.mark.parametrize("op", OPS)
+def test_lazily_negated_gradients(cuda_device, op):
+    """An incoming gradient with the negative bit counts with its sign (the bits are the negated ones')."""
+    out, inputs = _graph(op, cuda_device)
+    g = torch.randn_like(out)
+    want = torch.autograd.grad(out, inputs, -g, retain_graph=True)
+    got = torch.autograd.grad(out, inputs, torch._neg_view(g))
+    assert all(torch.equal(a, b) and a.any() for a, b in zip(got, want))
