@@ -48,6 +48,7 @@ def _empty_sparse_grad(weights):
 def _limited(grad, max_norm):
     """``grad`` scaled down to a 2-norm of at most ``max_norm``: a new tensor, since autograd may hand the
     same gradient to others."""
+    grad = grad.resolve_neg()
     if not gradient_clipping._dense(grad):
         grad = grad.contiguous()
     out = torch.empty_like(grad)

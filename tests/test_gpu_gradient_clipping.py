@@ -287,3 +287,18 @@ def test_max_grad_norm_of_the_tables(cuda_device, fp16, optimizer):
     one = torch.ones((), device=cuda_device, dtype=go.dtype).expand(B, T, D)  # out.sum().backward()
     got, want = trained(one, max_grad_norm=2.0), trained(one.contiguous(), max_grad_norm=2.0)
     assert torch.equal(got[0], want[0])
+
+
+def test_max_grad_norm_of_a_lazily_negated_gradient(cuda_device):
+    """A gradient with the negative bit is limited like any other."""
+    idx = torch.arange(6, dtype=torch.int32, device=cuda_device)
+    off = torch.arange(0, 7, 2, dtype=torch.int32, device=cuda_device)
+    go = torch.randn(3, 1, 8, device=cuda_device)
+    w0 = torch.randn(10, 8, device=cuda_device)
+    rows = []
+    for grad in (-go, torch._neg_view(go)):
+        m = ops.TableBatchedEmbeddingBags(1, 10, 8, learning_rate=0.5, max_grad_norm=0.25).cuda()
+        m.embedding_weights.data.copy_(w0)
+        m(idx, off).backward(grad)
+        rows.append(m.embedding_weights.detach().clone())
+    assert torch.equal(rows[0], rows[1]) and not torch.equal(rows[0], w0)
