@@ -60,7 +60,12 @@ int dtype_of(const Tensor& t) {
 }
 at::ScalarType weights_type(const Tensor& rows) { return rows.scalar_type() == at::kDouble ? at::kDouble : at::kFloat; }
 
+// Forward-mode differentiation keeps a tangent beside the tensor; what the kernels compute would come without one,
+// which means a derivative of zero.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+
 void check_cuda(const char* name, const Tensor& t) {
+  REQUIRE(!has_tangent(t), name, " carries a forward-mode tangent: there is no forward-mode derivative here");
   REQUIRE(t.defined() && t.is_cuda() && t.layout() == at::kStrided, name,
           " must be a CUDA tensor (this library has no CPU path)");
   REQUIRE(!t.is_neg(), name, " is a lazily negated view: call resolve_neg() on it");
@@ -82,7 +87,10 @@ int32_t* ints(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
 void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // An upstream gradient as the kernels read it: they see memory, not the negative bit that autograd may have set.
-Tensor incoming(const Tensor& grad) { return grad.detach().resolve_neg(); }
+Tensor incoming(const Tensor& grad) {
+  REQUIRE(!has_tangent(grad), "the gradient carries a forward-mode tangent: there is no forward-mode derivative here");
+  return grad.detach().resolve_neg();
+}
 
 // What a backward returns when its own graph is recorded: differentiating it again raises.
 variable_list once(variable_list grads) {
@@ -294,6 +302,7 @@ struct List {
     for (const auto& entry : tensors) {
       if (!entry.has_value()) continue;
       const Tensor& t = *entry;
+      REQUIRE(!has_tangent(t), "tensors carry a forward-mode tangent: there is no forward-mode derivative here");
       REQUIRE(t.defined() && t.is_cuda(), "tensors must be CUDA tensors (this library has no CPU path)");
       REQUIRE(t.layout() == at::kStrided && dtype_of(t) >= 0,
               "tensors must be dense float16, bfloat16, float32 or float64 tensors");
@@ -351,6 +360,7 @@ Tensor clip_grad_norm(const std::vector<std::optional<Tensor>>& tensors, double 
     const Tensor& t = *tensors[i];
     if (out) {
       const auto& o = (*out)[i];
+      REQUIRE(!o.has_value() || !has_tangent(*o), "out carries a forward-mode tangent: there is no forward-mode derivative here");
       REQUIRE(o.has_value() && o->defined() && o->layout() == at::kStrided && !o->is_neg() && o->device() == t.device() &&
                   o->scalar_type() == t.scalar_type() && o->sizes() == t.sizes() && same_order(*o, t),
               "out must match tensors in device, type, shape and strides");

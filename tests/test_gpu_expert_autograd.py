@@ -1,14 +1,16 @@
-"""Gradients of the routing operators where digits cancel.
+"""Gradients of the routing operators where digits cancel, and with gradients and inputs of unusual kinds.
 
 Tolerances count roundings (u = 2^-24), as in the tests of the operators themselves.
 """
 import numpy as np
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 import routing_testlib as ref
 from routing_testlib import assert_within, f64, unit
 from sparse_ads_baselines_b200 import expert_routing as er
+from sparse_ads_baselines_b200 import gradient_clipping as gc
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +68,25 @@ def test_lazily_negated_gradients(cuda_device, op):
     want = torch.autograd.grad(out, inputs, -g, retain_graph=True)
     got = torch.autograd.grad(out, inputs, torch._neg_view(g))
     assert all(torch.equal(a, b) and a.any() for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("op", OPS)
+def test_forward_mode_over_a_backward_is_refused(cuda_device, op):
+    """A gradient with a tangent would come back without one, which says that its derivative is zero."""
+    out, inputs = _graph(op, cuda_device)
+    with fwd.dual_level():
+        g = fwd.make_dual(torch.ones_like(out), torch.ones_like(out))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(out, inputs, g, retain_graph=True)
+    assert all(t.isfinite().all() for t in torch.autograd.grad(out, inputs, torch.ones_like(out)))
+
+
+def test_forward_mode_weights_and_out_are_refused(cuda_device):
+    x, y, w = torch.randn(4, 6, device=cuda_device), torch.randn(8, 6, device=cuda_device), torch.rand(4, 2, device=cuda_device)
+    p = er.plan(torch.arange(8, dtype=torch.int32, device=cuda_device).view(4, 2) % 3, 3)
+    with fwd.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            er.combine(y, p, fwd.make_dual(w, torch.ones_like(w)))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            gc.clip_grad_norm([x], 1.0, out=[fwd.make_dual(torch.zeros_like(x), torch.ones_like(x))])
+    er.combine(y, p, w)
