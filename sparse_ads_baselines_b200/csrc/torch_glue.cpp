@@ -8,10 +8,12 @@
 #include <pybind11/stl.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
@@ -60,6 +62,14 @@ int dtype_of(const Tensor& t) {
 }
 at::ScalarType weights_type(const Tensor& rows) { return rows.scalar_type() == at::kDouble ? at::kDouble : at::kFloat; }
 
+// A recorder sees the allocation of an output but not the kernel that fills it: what it records returns memory that
+// nobody wrote.
+void refuse_recording() {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  REQUIRE(!torch::jit::tracer::isTracing() && !Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+          "expert routing and gradient clipping cannot be recorded (torch.jit.trace, make_fx, torch.export)");
+}
+
 // Forward-mode differentiation keeps a tangent beside the tensor; what the kernels compute would come without one,
 // which means a derivative of zero.
 bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
@@ -88,6 +98,7 @@ void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // An upstream gradient as the kernels read it: they see memory, not the negative bit that autograd may have set.
 Tensor incoming(const Tensor& grad) {
+  refuse_recording();
   REQUIRE(!has_tangent(grad), "the gradient carries a forward-mode tangent: there is no forward-mode derivative here");
   return grad.detach().resolve_neg();
 }
@@ -147,6 +158,7 @@ struct Gate : Function<Gate> {
 };
 
 std::tuple<Tensor, Tensor> gate(const Tensor& logits, int64_t k, bool renormalize) {
+  refuse_recording();
   check_rows("logits", logits);
   REQUIRE(logits.size(1) <= kMaxExperts, "logits must be [N, E] with E in 1..", kMaxExperts);
   REQUIRE(k >= 1 && k <= std::min(logits.size(1), kMaxChoices), "k must be in 1..min(E, ", kMaxChoices, "), got ", k);
@@ -157,6 +169,7 @@ std::tuple<Tensor, Tensor> gate(const Tensor& logits, int64_t k, bool renormaliz
 
 // ---------------------------------------------------------------- plan
 std::tuple<Tensor, Tensor, Tensor> plan(const Tensor& choices, int64_t num_experts) {
+  refuse_recording();
   check_int32("experts", choices);
   REQUIRE(choices.dim() == 2 && choices.size(1) > 0, "experts must be [N, k]");
   REQUIRE(num_experts >= 1 && num_experts <= kMaxExperts, "num_experts must be in 1..", kMaxExperts, ", got ", num_experts);
@@ -262,6 +275,7 @@ struct Combine : Function<Combine> {
 };
 
 Tensor dispatch(const Tensor& x, const Tensor& offsets, const Tensor& positions) {
+  refuse_recording();
   check_rows("x", x);
   check_plan(offsets, positions, x);
   REQUIRE(x.size(0) == positions.size(0), "x has ", x.size(0), " rows but the plan was made for ", positions.size(0));
@@ -270,6 +284,7 @@ Tensor dispatch(const Tensor& x, const Tensor& offsets, const Tensor& positions)
 }
 
 Tensor combine(const Tensor& y, const Tensor& offsets, const Tensor& positions, const std::optional<Tensor>& weights) {
+  refuse_recording();
   check_rows("y", y);
   check_plan(offsets, positions, y);
   const int64_t N = positions.size(0), k = positions.size(1);
@@ -331,6 +346,7 @@ Tensor norm_workspace(const List& list) {
 }
 
 Tensor grad_norm(const std::vector<std::optional<Tensor>>& tensors) {
+  refuse_recording();
   const List list(tensors);
   if (!list.first) return no_norm();
   const c10::cuda::CUDAGuard guard(list.first->device());
@@ -349,6 +365,7 @@ bool same_order(const Tensor& a, const Tensor& b) {
 
 Tensor clip_grad_norm(const std::vector<std::optional<Tensor>>& tensors, double max_norm, double eps,
                       const std::optional<std::vector<std::optional<Tensor>>>& out) {
+  refuse_recording();
   REQUIRE(max_norm >= 0 && eps >= 0, "max_norm and eps must not be negative");
   const List list(tensors);
   if (out) REQUIRE(out->size() == tensors.size(), "out must have as many entries as tensors");

@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import routing_testlib as ref
 from routing_testlib import assert_within, f64, unit
@@ -90,3 +91,18 @@ def test_forward_mode_weights_and_out_are_refused(cuda_device):
         with pytest.raises(RuntimeError, match="forward-mode"):
             gc.clip_grad_norm([x], 1.0, out=[fwd.make_dual(torch.zeros_like(x), torch.ones_like(x))])
     er.combine(y, p, w)
+
+
+def test_recording_is_refused(cuda_device):
+    x = torch.randn(4, 6, device=cuda_device)
+    for f in (lambda t: er.gate(t, 2)[0], lambda t: er.gate(t.requires_grad_(), 2)[0], lambda t: gc.clip_grad_norm([t], 1.0)):
+        with pytest.raises(RuntimeError, match="recorded"):
+            torch.jit.trace(f, x.clone(), check_trace=False)
+        with pytest.raises(RuntimeError, match="recorded"):
+            make_fx(f)(x.clone())
+    out, inputs = _graph("gate", cuda_device)
+    with pytest.raises(RuntimeError, match="recorded"):
+        make_fx(lambda g: torch.autograd.grad(out, inputs, g, retain_graph=True)[0])(torch.ones_like(out))
+    # a compiled function leaves the recorder around the call
+    compiled = torch.compile(lambda t: er.gate(t * 2, 2)[0] * 3, backend="eager")
+    assert torch.equal(compiled(x), er.gate(x * 2, 2)[0] * 3)

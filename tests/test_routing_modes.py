@@ -3,6 +3,7 @@ computed there is refused before anything else is looked at."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from sparse_ads_baselines_b200 import expert_routing as er
 from sparse_ads_baselines_b200 import gradient_clipping as gc
@@ -31,3 +32,25 @@ def test_forward_mode_is_refused(call):
             _calls(lambda t: fwd.make_dual(t, torch.ones_like(t)))[call]()
     with pytest.raises(RuntimeError, match="CUDA tensor"):  # the same call without a tangent
         _calls(lambda t: t)[call]()
+
+
+RECORDED = {
+    "gate": lambda x: er.gate(x, 2)[0],
+    "plan": lambda x: er.plan(x.int(), 3).order,
+    "dispatch": lambda x: er.dispatch(x, _plan(x.device)),
+    "combine": lambda x: er.combine(x.repeat(2, 1), _plan(x.device)),
+    "grad_norm": lambda x: gc.grad_norm([x]),
+    "clip_grad_norm": lambda x: gc.clip_grad_norm([x], 1.0),
+    "clip_grad_norm out": lambda x: gc.clip_grad_norm([x], 1.0, out=[torch.empty_like(x)]),
+}
+RECORDERS = {"trace": lambda f, x: torch.jit.trace(f, x, check_trace=False), "make_fx": lambda f, x: make_fx(f)(x)}
+
+
+@pytest.mark.parametrize("recorder", RECORDERS)
+@pytest.mark.parametrize("op", RECORDED)
+def test_recording_is_refused(op, recorder):
+    """A recorder would keep the allocation of the result and nothing of what fills it."""
+    with pytest.raises(RuntimeError, match="recorded"):
+        RECORDERS[recorder](RECORDED[op], torch.zeros(4, 6))
+    with pytest.raises(RuntimeError, match="CUDA tensor"):  # and not refused once the recorder is gone
+        RECORDED[op](torch.zeros(4, 6))
