@@ -84,22 +84,42 @@ __device__ __forceinline__ double sum_squares(const Raw<VB>& r) {
   return d;
 }
 
+// How the summing pass loads: ReadOnly where the kernel writes none of the tensors, Ordinary where it goes on to scale
+// them (the read-only path is only for memory that nothing writes while the kernel runs).
+struct ReadOnly {
+  template <typename T>
+  __device__ static __forceinline__ Raw<sizeof(T)> one(const T* p) {
+    return ld_stream<sizeof(T)>(p);
+  }
+  __device__ static __forceinline__ Raw<16> vector(const void* p, uint64_t policy) { return ld_stream_hint<16>(p, policy); }
+};
+struct Ordinary {
+  template <typename T>
+  __device__ static __forceinline__ Raw<sizeof(T)> one(const T* p) {
+    const T v = *p;
+    Raw<sizeof(T)> r;
+    memcpy(&r, &v, sizeof(T));
+    return r;
+  }
+  __device__ static __forceinline__ Raw<16> vector(const void* p, uint64_t policy) { return ld_rw_hint<16>(p, policy); }
+};
+
 // By `threads` threads of which this one is `me`.
-template <typename T>
+template <typename LOADS, typename T>
 __device__ double chunk_squares(const T* p, int n, int me, int threads, uint64_t policy) {
   constexpr int NV = 16 / sizeof(T), U = 4;
   const int head = min(n, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / static_cast<int>(sizeof(T)));
   const int nvec = (n - head) / NV, tail = head + nvec * NV;
   double s = 0.0;
-  for (int i = me; i < head; i += threads) s += sum_squares<T, sizeof(T)>(ld_stream<sizeof(T)>(p + i));
-  for (int i = tail + me; i < n; i += threads) s += sum_squares<T, sizeof(T)>(ld_stream<sizeof(T)>(p + i));
+  for (int i = me; i < head; i += threads) s += sum_squares<T, sizeof(T)>(LOADS::one(p + i));
+  for (int i = tail + me; i < n; i += threads) s += sum_squares<T, sizeof(T)>(LOADS::one(p + i));
   const T* q = p + head;
   for (int v = me; v < nvec; v += threads * U) {
     Raw<16> r[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = v + u * threads;
-      r[u] = i < nvec ? ld_stream_hint<16>(q + static_cast<int64_t>(i) * NV, policy) : raw_none<16>();
+      r[u] = i < nvec ? LOADS::vector(q + static_cast<int64_t>(i) * NV, policy) : raw_none<16>();
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) s += sum_squares<T, 16>(r[u]);
@@ -137,14 +157,14 @@ __device__ __forceinline__ Piece piece_of(const Table<CAP>& t, int c, int chunk,
   return p;
 }
 
-template <int CAP>
+template <typename LOADS, int CAP>
 __device__ __forceinline__ double piece_squares(const Table<CAP>& t, const Piece& p, int me, int threads, uint64_t policy) {
   const void* src = t.src[p.tensor];
   switch (t.dtype[p.tensor]) {
-    case TBE_F16: return chunk_squares(static_cast<const __half*>(src) + p.at, p.n, me, threads, policy);
-    case TBE_BF16: return chunk_squares(static_cast<const __nv_bfloat16*>(src) + p.at, p.n, me, threads, policy);
-    case TBE_F32: return chunk_squares(static_cast<const float*>(src) + p.at, p.n, me, threads, policy);
-    default: return chunk_squares(static_cast<const double*>(src) + p.at, p.n, me, threads, policy);
+    case TBE_F16: return chunk_squares<LOADS>(static_cast<const __half*>(src) + p.at, p.n, me, threads, policy);
+    case TBE_BF16: return chunk_squares<LOADS>(static_cast<const __nv_bfloat16*>(src) + p.at, p.n, me, threads, policy);
+    case TBE_F32: return chunk_squares<LOADS>(static_cast<const float*>(src) + p.at, p.n, me, threads, policy);
+    default: return chunk_squares<LOADS>(static_cast<const double*>(src) + p.at, p.n, me, threads, policy);
   }
 }
 
@@ -154,7 +174,7 @@ __global__ void __launch_bounds__(kClipThreads) grad_norm_kernel(const __grid_co
   const uint64_t pass = l2_policy_evict_first(), stay = l2_policy_evict_normal();
   double s = 0.0;
   for (int c = blockIdx.x; c < t.chunks; c += gridDim.x)
-    s += piece_squares(t, piece_of(t, c, kChunk, tensor_of(t, c)), threadIdx.x, kClipThreads, c < keep ? pass : stay);
+    s += piece_squares<ReadOnly>(t, piece_of(t, c, kChunk, tensor_of(t, c)), threadIdx.x, kClipThreads, c < keep ? pass : stay);
   s = block_sum(s);
   if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
@@ -277,10 +297,10 @@ __global__ void __launch_bounds__(1024) grad_clip_small_kernel(const __grid_cons
   Piece own_piece{0, 0, 0};  // the first of this warp's pieces, which is all it has unless the list is long
   if (first < t.chunks) {
     own_piece = piece_of(t, first, kSmallChunk, owners.tensor[first]);
-    s = piece_squares(t, own_piece, lane, 32, policy);
+    s = piece_squares<Ordinary>(t, own_piece, lane, 32, policy);
   }
   for (int c = first + step; c < t.chunks; c += step)
-    s += piece_squares(t, piece_of(t, c, kSmallChunk, owners.tensor[c]), lane, 32, policy);
+    s += piece_squares<Ordinary>(t, piece_of(t, c, kSmallChunk, owners.tensor[c]), lane, 32, policy);
 #pragma unroll
   for (int m = 1; m < 32; m <<= 1) s += __shfl_xor_sync(kFullMask, s, m);
   if (lane == 0) part[warp] = s;
