@@ -304,7 +304,7 @@ TBE_API int tbe_sort_segments(const int32_t* table_offsets, const int32_t* indic
 
 /* For models whose samples pass through a few of E experts.  The reference has no such layer.  dtype is
  * any tbe_dtype_t; "weights" and their gradients are fp32 (fp64 for TBE_F64).  All arrays are device
- * memory.  Rows may have any width; they move in the widest vectors (16 bytes down to one element) that
+ * memory, aligned to their elements (checked).  Rows may have any width; they move in the widest vectors (16 bytes down to one element) that
  * the addresses and strides allow.  Limits: E <= 1024, k <= min(E, 32) in the gate, N*k <= 2^31 - 1025.
  *
  * tbe_expert_gate: logits [N][E] (rows row_stride elements apart) -> the k largest of every row,

@@ -108,7 +108,9 @@ __device__ __forceinline__ Raw<VB> narrow(const typename Acc<T>::type* in) {
   return r;
 }
 
+// Bytes of an element, and of a weight or a sum beside it.
 inline int any_elem_size(int dtype) { return dtype == TBE_BF16 ? 2 : elem_size(dtype); }
+inline int acc_size(int dtype) { return dtype == TBE_F64 ? 8 : 4; }
 inline bool known_dtype(int dtype) {
   return dtype == TBE_F32 || dtype == TBE_F16 || dtype == TBE_F64 || dtype == TBE_BF16;
 }
@@ -117,5 +119,11 @@ inline bool known_dtype(int dtype) {
 inline int vector_bytes_of(uint64_t bits) { return bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2; }
 
 inline uint64_t addr_bits(const void* p) { return static_cast<uint64_t>(reinterpret_cast<uintptr_t>(p)); }
+
+// Whether every address is a multiple of `size` (null is).  The entry points refuse what would fault on the GPU.
+template <typename... P>
+bool aligned_to(uint64_t size, P... p) {
+  return ((addr_bits(p) | ...) & (size - 1)) == 0;
+}
 
 }  // namespace tbe

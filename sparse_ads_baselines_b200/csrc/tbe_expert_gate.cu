@@ -584,6 +584,9 @@ int run_gate(const char* who, GateArgs a, int dtype, bool backward, cudaStream_t
   if (a.N == 0) return TBE_OK;
   TBE_REQUIRE(a.logits && a.weights && a.experts, "%s: null pointer argument", who);
   TBE_REQUIRE(!backward || (a.grad_weights && a.grad_logits), "%s: null pointer argument", who);
+  TBE_REQUIRE(aligned_to(any_elem_size(dtype), a.logits, a.grad_logits) &&
+                  aligned_to(acc_size(dtype), a.weights, a.grad_weights) && aligned_to(4, a.experts),
+              "%s: a pointer is not aligned to its elements", who);
   // lanes per row: eight values each (the narrowest group reads 16-bit rows as whole vectors), and a lane
   // for every slot
   a.glog = 0;

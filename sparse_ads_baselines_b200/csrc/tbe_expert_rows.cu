@@ -559,6 +559,8 @@ extern "C" int tbe_expert_plan(const int32_t* experts, int32_t* offsets, int32_t
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(TBE_ERR_WORKSPACE_TOO_SMALL, "tbe_expert_plan: workspace of %lld bytes, %lld needed",
                 static_cast<long long>(workspace_bytes), static_cast<long long>(need));
+  TBE_REQUIRE(aligned_to(4, experts, offsets, positions, order, workspace),
+              "tbe_expert_plan: a pointer is not aligned to its elements");
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   const PlanShape s = plan_shape(M);
   int bits = 1;
@@ -608,6 +610,8 @@ extern "C" int tbe_expert_dispatch(const void* x, int64_t row_stride, const int3
   TBE_REQUIRE(x && positions && offsets && y, "tbe_expert_dispatch: null pointer argument");
   TBE_REQUIRE(E > 0 && (N == 1 || row_stride >= 0), "tbe_expert_dispatch: E must be > 0, row_stride >= 0");
   const int64_t es = any_elem_size(dtype);
+  TBE_REQUIRE(aligned_to(es, x, y) && aligned_to(4, positions, offsets),
+              "tbe_expert_dispatch: a pointer is not aligned to its elements");
   RowArgs a{};
   a.x = static_cast<const char*>(x);
   a.x_stride = N == 1 ? 0 : row_stride * es;
@@ -633,6 +637,9 @@ extern "C" int tbe_expert_combine(const void* y, const int32_t* positions, const
   if (N == 0) return TBE_OK;
   TBE_REQUIRE(y && positions && offsets && out, "tbe_expert_combine: null pointer argument");
   TBE_REQUIRE(E > 0, "tbe_expert_combine: E must be > 0");
+  TBE_REQUIRE(aligned_to(any_elem_size(dtype), y, out) && aligned_to(acc_size(dtype), weights) &&
+                  aligned_to(4, positions, offsets),
+              "tbe_expert_combine: a pointer is not aligned to its elements");
   RowArgs a{};
   a.x = static_cast<const char*>(y);
   a.row_bytes = a.x_stride = D * any_elem_size(dtype);
@@ -663,6 +670,9 @@ extern "C" int tbe_expert_combine_backward(const void* grad_out, int64_t grad_st
               "tbe_expert_combine_backward: null pointer argument");
   TBE_REQUIRE(E > 0 && (N == 1 || grad_stride >= 0), "tbe_expert_combine_backward: E must be > 0, grad_stride >= 0");
   const int64_t es = any_elem_size(dtype);
+  TBE_REQUIRE(aligned_to(es, grad_out, y, grad_y) && aligned_to(acc_size(dtype), weights, grad_weights) &&
+                  aligned_to(4, positions, offsets),
+              "tbe_expert_combine_backward: a pointer is not aligned to its elements");
   GradArgs a{};
   a.grad_out = static_cast<const char*>(grad_out);
   a.go_stride = N == 1 ? 0 : grad_stride * es;

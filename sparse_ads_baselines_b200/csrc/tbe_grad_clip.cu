@@ -532,6 +532,7 @@ extern "C" int tbe_grad_norm(const void* const* tensors, const int64_t* numels, 
                              float* norm, void* workspace, int64_t workspace_bytes, void* stream_v) {
   using namespace tbe;
   TBE_REQUIRE(norm, "tbe_grad_norm: null pointer argument");
+  TBE_REQUIRE(aligned_to(4, norm), "tbe_grad_norm: norm is not aligned to its elements");
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   if (const int rc = check_list("tbe_grad_norm", tensors, numels, dtypes, count)) return rc;
   if (const int rc = check_workspace("tbe_grad_norm", count, workspace, workspace_bytes)) return rc;
@@ -552,6 +553,7 @@ extern "C" int tbe_grad_clip(const void* const* tensors, void* const* outputs, c
                              int64_t workspace_bytes, void* stream_v) {
   using namespace tbe;
   TBE_REQUIRE(norm && (count == 0 || outputs), "tbe_grad_clip: null pointer argument");
+  TBE_REQUIRE(aligned_to(4, norm), "tbe_grad_clip: norm is not aligned to its elements");
   TBE_REQUIRE(max_norm >= 0.0 && eps >= 0.0, "tbe_grad_clip: max_norm and eps must not be negative");
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   if (const int rc = check_list("tbe_grad_clip", tensors, numels, dtypes, count)) return rc;

@@ -82,6 +82,40 @@ def test_bad_arguments_of_the_c_entries(lib):
     refused(lib.tbe_grad_norm(odd, sizes, types, 1, p, ws, need, None), b"aligned")
 
 
+def test_misaligned_pointers_of_the_c_entries(lib):
+    """An address that is no multiple of its elements' size faults on the GPU; the host refuses it."""
+    buf = ctypes.create_string_buffer(1024)
+    p = (ctypes.addressof(buf) + 63) & ~63
+    types = [(_lib.TBE_F16, 2, 4), (_lib.TBE_BF16, 2, 4), (_lib.TBE_F32, 4, 4), (_lib.TBE_F64, 8, 8)]
+
+    def refused_one_by_one(call, sizes):
+        for i, size in enumerate(sizes):
+            args = [p] * len(sizes)
+            args[i] = p + size // 2
+            assert call(*args) == -1 and b"aligned" in lib.tbe_last_error_string(), (i, lib.tbe_last_error_string())
+
+    for t, es, ws in types:
+        refused_one_by_one(lambda x, w, e: lib.tbe_expert_gate(x, 4, w, e, 1, 4, 1, t, 1, None), [es, ws, 4])
+        for ren in (0, 1):
+            refused_one_by_one(lambda g, w, e, d: lib.tbe_expert_gate_backward(g, p, 4, w, e, d, 1, 4, 1, t, ren, None),
+                               [ws, ws, 4, es])
+        refused_one_by_one(lambda x: lib.tbe_expert_gate_backward(p, x, 4, p, p, p, 1, 4, 1, t, 0, None), [es])
+        refused_one_by_one(lambda x, q, o, y: lib.tbe_expert_dispatch(x, 4, q, o, y, 1, 1, 4, 2, t, None), [es, 4, 4, es])
+        refused_one_by_one(lambda y, q, o, w, d: lib.tbe_expert_combine(y, q, o, w, d, 1, 1, 4, 2, t, None),
+                           [es, 4, 4, ws, es])
+        refused_one_by_one(
+            lambda g, y, q, o, w, dy, dw: lib.tbe_expert_combine_backward(g, 4, y, q, o, w, dy, dw, 1, 1, 4, 2, t, None),
+            [es, es, 4, 4, ws, es, ws])
+    refused_one_by_one(lambda e, o, q, r: lib.tbe_expert_plan(e, o, q, r, 8, 4, None, 0, None), [4] * 4)
+    need = lib.tbe_expert_plan_workspace_bytes(200_000, 4)
+    refused_one_by_one(lambda w: lib.tbe_expert_plan(p, p, p, p, 200_000, 4, w, need, None), [4])
+    ptrs, one = (ctypes.c_void_p * 1)(p), (ctypes.c_void_p * 1)(p + 64)
+    sizes, kinds = (ctypes.c_int64 * 1)(4), (ctypes.c_int32 * 1)(_lib.TBE_F32)
+    need = lib.tbe_grad_norm_workspace_bytes(1)
+    refused_one_by_one(lambda n, w: lib.tbe_grad_norm(ptrs, sizes, kinds, 1, n, w, need, None), [4, 8])
+    refused_one_by_one(lambda n, w: lib.tbe_grad_clip(ptrs, one, sizes, kinds, 1, 1.0, 0.0, n, w, need, None), [4, 8])
+
+
 def test_dense_memory_is_recognised():
     a = torch.zeros(4, 6, 5)
     assert all(gc._dense(t) for t in (a, a.permute(2, 0, 1), a[:1], a[2:3, 1:2], torch.zeros(()), torch.zeros(0, 3)))
