@@ -313,7 +313,7 @@ TBE_API int tbe_sort_segments(const int32_t* table_offsets, const int32_t* indic
  * A logit of -inf is never chosen: its slot gets id -1 and weight 0 (a row of nothing else: all -1, all
  * 0).  NaN ranks above +inf; a row with a chosen NaN or +inf (renormalize = 0: with any) has NaN weights.
  * tbe_expert_gate_backward: grad_logits [N][E] (contiguous) from grad_weights [N][k], the gate's
- * results and (read only when renormalize = 0) its logits. */
+ * results and, when renormalize = 0, its logits; else logits and row_stride are ignored (logits may be NULL). */
 TBE_API int tbe_expert_gate(const void* logits, int64_t row_stride, void* weights, int32_t* experts, int64_t N,
                             int64_t E, int64_t k, int dtype, int renormalize, void* stream);
 TBE_API int tbe_expert_gate_backward(const void* grad_weights, const void* logits, int64_t row_stride,

@@ -575,6 +575,11 @@ int launch_gate_type(const GateArgs& a, bool backward, cudaStream_t stream) {
 }
 
 int run_gate(const char* who, GateArgs a, int dtype, bool backward, cudaStream_t stream) {
+  const bool reads_logits = !(backward && a.renormalize);
+  if (!reads_logits) {  // nor do they decide anything
+    a.logits = nullptr;
+    a.stride = 0;
+  }
   TBE_REQUIRE(a.N < (1ll << 31), "%s: N must be below 2^31", who);
   TBE_REQUIRE(a.N >= 0 && a.E > 0 && a.E <= kGateMaxExperts, "%s: the number of experts must be 1..%d", who,
               kGateMaxExperts);
@@ -582,7 +587,7 @@ int run_gate(const char* who, GateArgs a, int dtype, bool backward, cudaStream_t
   TBE_REQUIRE(known_dtype(dtype), "%s: bad dtype %d", who, dtype);
   TBE_REQUIRE(a.N <= 1 || a.stride >= 0, "%s: negative row stride", who);
   if (a.N == 0) return TBE_OK;
-  TBE_REQUIRE(a.logits && a.weights && a.experts, "%s: null pointer argument", who);
+  TBE_REQUIRE((a.logits || !reads_logits) && a.weights && a.experts, "%s: null pointer argument", who);
   TBE_REQUIRE(!backward || (a.grad_weights && a.grad_logits), "%s: null pointer argument", who);
   TBE_REQUIRE(aligned_to(any_elem_size(dtype), a.logits, a.grad_logits) &&
                   aligned_to(acc_size(dtype), a.weights, a.grad_weights) && aligned_to(4, a.experts),

@@ -149,10 +149,10 @@ struct Gate : Function<Gate> {
     const int64_t N = weights.size(0), k = weights.size(1), E = ctx->saved_data["experts"].toInt();
     Tensor out = at::empty({N, E}, weights.options().dtype(static_cast<at::ScalarType>(ctx->saved_data["dtype"].toInt())));
     const bool renormalize = !saved[2].defined();
-    const Tensor rows = renormalize ? out : dense_rows(saved[2].detach());
+    const Tensor rows = renormalize ? Tensor() : dense_rows(saved[2].detach());
     must("tbe_expert_gate_backward",
-         tbe_expert_gate_backward(g.data_ptr(), rows.data_ptr(), rows.stride(0), weights.data_ptr(), ints(experts),
-                                  out.data_ptr(), N, E, k, dtype_of(out), renormalize, stream_of(out)));
+         tbe_expert_gate_backward(g.data_ptr(), data(rows), renormalize ? 0 : rows.stride(0), weights.data_ptr(),
+                                  ints(experts), out.data_ptr(), N, E, k, dtype_of(out), renormalize, stream_of(out)));
     return once({out, Tensor(), Tensor()});
   }
 };

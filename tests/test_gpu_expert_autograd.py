@@ -2,6 +2,8 @@
 
 Tolerances count roundings (u = 2^-24), as in the tests of the operators themselves.
 """
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -10,6 +12,7 @@ from torch.fx.experimental.proxy_tensor import make_fx
 
 import routing_testlib as ref
 from routing_testlib import assert_within, f64, unit
+from sparse_ads_baselines_b200 import _lib
 from sparse_ads_baselines_b200 import expert_routing as er
 from sparse_ads_baselines_b200 import gradient_clipping as gc
 
@@ -106,3 +109,20 @@ def test_recording_is_refused(cuda_device):
     # a compiled function leaves the recorder around the call
     compiled = torch.compile(lambda t: er.gate(t * 2, 2)[0] * 3, backend="eager")
     assert torch.equal(compiled(x), er.gate(x * 2, 2)[0] * 3)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, torch.float64])
+def test_renormalized_gradient_without_logits(cuda_device, dtype):
+    """The C entry takes no logits, or any, where it does not read them."""
+    torch.manual_seed(5)
+    x = torch.randn(33, 48, device=cuda_device, dtype=dtype, requires_grad=True)
+    w, e = er.gate(x, 4)
+    g = torch.randn_like(w)
+    want, = torch.autograd.grad(w, x, g)
+    kind = {torch.bfloat16: _lib.TBE_BF16, torch.float32: _lib.TBE_F32, torch.float64: _lib.TBE_F64}[dtype]
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    for logits, stride in ((None, 0), (None, -1), (x.data_ptr() + 1, 7)):
+        out = torch.full_like(x, float("nan"))
+        _lib.call("tbe_expert_gate_backward", g.data_ptr(), logits, stride, w.data_ptr(), e.data_ptr(), out.data_ptr(),
+                  33, 48, 4, kind, 1, stream)
+        assert torch.equal(out, want)

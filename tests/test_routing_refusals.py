@@ -116,6 +116,19 @@ def test_misaligned_pointers_of_the_c_entries(lib):
     refused_one_by_one(lambda n, w: lib.tbe_grad_clip(ptrs, one, sizes, kinds, 1, 1.0, 0.0, n, w, need, None), [4, 8])
 
 
+def test_the_gates_renormalized_gradient_needs_no_logits(lib):
+    """As the header says: a call is refused for what it reads."""
+    buf = ctypes.create_string_buffer(256)
+    p = (ctypes.addressof(buf) + 63) & ~63
+    for logits, stride in ((None, 4), (p + 1, 4), (p, -4)):
+        rc = lib.tbe_expert_gate_backward(p, logits, stride, p, p, p, 2, 4, 1, _lib.TBE_F32, 0, None)
+        assert rc == -1  # the other gradient reads them
+        rc = lib.tbe_expert_gate_backward(p, logits, stride, p, p, p, 0, 4, 1, _lib.TBE_F32, 1, None)
+        assert rc == 0, lib.tbe_last_error_string()
+        rc = lib.tbe_expert_gate_backward(p, logits, stride, p, p, None, 2, 4, 1, _lib.TBE_F32, 1, None)
+        assert rc == -1 and b"null" in lib.tbe_last_error_string()
+
+
 def test_dense_memory_is_recognised():
     a = torch.zeros(4, 6, 5)
     assert all(gc._dense(t) for t in (a, a.permute(2, 0, 1), a[:1], a[2:3, 1:2], torch.zeros(()), torch.zeros(0, 3)))
