@@ -5,7 +5,7 @@ compiled to an object file (in parallel, skipped when up to date) and linked int
 ``sparse_ads_baselines_b200/libtbe_b200.so``; the CUDA runtime is linked statically so the library
 depends on nothing but the driver.  ``csrc/torch_glue.cpp`` -- the PyTorch side of expert routing and
 gradient clipping -- becomes the extension module ``_torch_glue.so`` beside it, linked to that library and
-to the PyTorch that builds it.
+to the PyTorch that builds it; without PyTorch it is left out.
 """
 import concurrent.futures
 import os
@@ -44,7 +44,11 @@ def _newer(target, deps):
 
 
 def _build_glue(force):
-    import torch
+    try:
+        import torch
+    except ImportError as e:  # a host without PyTorch binds the C library
+        sys.stderr.write("PyTorch cannot be imported (%s): _torch_glue.so is not built\n" % e)
+        return
     from torch.utils import cpp_extension
     src = os.path.join(CSRC, "torch_glue.cpp")
     header = os.path.join(HERE, "..", "include", "tbe_b200.h")
