@@ -11,7 +11,7 @@
 #include <sys/mman.h>
 #include <utility>
 
-#include "tbe_common.cuh"
+#include "tbe_elem.cuh"
 
 namespace tbe {
 namespace {
@@ -21,9 +21,10 @@ std::atomic<int64_t> g_library_launches{0};
 std::atomic<int> g_tuning[kTuneCount];
 const char* const kTuningNames[kTuneCount] = {"fwd_unroll", "fwd_threads", "bwd_threads", "bwd_unroll",
                                               "long_segment", "fwd_blocks_per_sm", "bwd_blocks_per_sm", "bwd_vpl",
-                                              "bwd_sort", "sort_bucket", "split_runs", "bwd_stride",
-                                              "row_threads"};
+                                              "bwd_sort", "sort_bucket", "split_runs", "bwd_stride"};
 }  // namespace
+
+std::atomic<int> g_row_threads{0};
 
 namespace {
 struct TimedLaunch {
@@ -115,6 +116,10 @@ extern "C" int tbe_set_tuning(const char* name, int value) {
       tbe::g_tuning[i].store(value);
       return TBE_OK;
     }
+  }
+  if (std::strcmp(name, "row_threads") == 0) {
+    tbe::g_row_threads.store(value);
+    return TBE_OK;
   }
   return tbe::fail(TBE_ERR_INVALID_ARGUMENT, "tbe_set_tuning: unknown knob '%s'", name);
 }

@@ -36,7 +36,6 @@ enum Tuning {
   kTuneSortBucket,  // wanted mean bucket size of the two-level sort (0: default)
   kTuneSplitRuns,   // 1: never cut long runs into parts (one CTA per queued run)
   kTuneBwdStride,   // run_kernel's warps walk the tiles 1: with a fixed stride, 2: by ticket, 0: by the gradient's size
-  kTuneRowThreads,  // most threads per launch of dispatch / combine (0: as many as 32-bit indices allow)
   kTuneCount
 };
 

@@ -8,9 +8,14 @@
 #include <cuda_bf16.h>
 #include <string.h>
 
+#include <atomic>
+
 #include "tbe_common.cuh"
 
 namespace tbe {
+
+// The knob "row_threads": most threads per launch of dispatch / combine (0: as many as 32-bit indices allow).
+extern std::atomic<int> g_row_threads;
 
 template <>
 struct Raw<4> {

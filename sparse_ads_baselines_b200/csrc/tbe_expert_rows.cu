@@ -424,7 +424,7 @@ int per_sample_launches(const char* name, RowArgs a, int64_t N, int vb, int u, c
   a.nvec = static_cast<uint32_t>(a.row_bytes / vb);
   a.per_row = a.nvec >= 32u * u ? (a.nvec + 32 * u - 1) / (32 * u) * 32 : (a.nvec + u - 1) / u;
   a.div = make_fastdiv(a.per_row);
-  const int64_t knob = tuning(kTuneRowThreads), most = knob > 0 ? knob : 0xffffffffll - 4096;
+  const int64_t knob = g_row_threads.load(std::memory_order_relaxed), most = knob > 0 ? knob : 0xffffffffll - 4096;
   const int64_t step = most > a.per_row ? most / a.per_row : 1;  // per_row <= 2^28
   for (int64_t n0 = 0; n0 < N; n0 += step) {
     const int64_t n = N - n0 < step ? N - n0 : step;
