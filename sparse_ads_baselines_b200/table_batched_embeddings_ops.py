@@ -109,7 +109,10 @@ class TableBatchedEmbeddingBags(nn.Module):
 
     ``max_grad_norm`` (None: no limit) scales the gradient of the returned ``[B, T, D]`` down to this 2-norm
     before the fused optimizer uses it; the gradient of ``per_sample_weights`` is taken from the scaled one.
+    The sharded, cached and mixed-width modules have no such limit.
     """
+
+    max_grad_norm = None  # of modules that were saved without one
 
     def __init__(self, num_tables, num_embeddings, embedding_dim, optimizer=Optimizer.SGD, learning_rate=0.01,
                  eps=None, stochastic_rounding=False, fp16=False, managed=EmbeddingLocation.DEVICE, *,
