@@ -12,6 +12,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
@@ -71,11 +72,13 @@ void refuse_recording() {
 }
 
 // Forward-mode differentiation keeps a tangent beside the tensor; what the kernels compute would come without one,
-// which means a derivative of zero.
+// which means a derivative of zero.  Tangents exist inside a dual_level() only; asking a view for one takes two locks
+// (2 us for 40 tensors), so the level is asked first.
+bool in_forward_mode() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
 bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
 
 void check_cuda(const char* name, const Tensor& t) {
-  REQUIRE(!has_tangent(t), name, " carries a forward-mode tangent: there is no forward-mode derivative here");
+  REQUIRE(!in_forward_mode() || !has_tangent(t), name, " carries a forward-mode tangent: there is no forward-mode derivative here");
   REQUIRE(t.defined() && t.is_cuda() && t.layout() == at::kStrided, name,
           " must be a CUDA tensor (this library has no CPU path)");
   REQUIRE(!t.is_neg(), name, " is a lazily negated view: call resolve_neg() on it");
@@ -99,7 +102,7 @@ void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 // An upstream gradient as the kernels read it: they see memory, not the negative bit that autograd may have set.
 Tensor incoming(const Tensor& grad) {
   refuse_recording();
-  REQUIRE(!has_tangent(grad), "the gradient carries a forward-mode tangent: there is no forward-mode derivative here");
+  REQUIRE(!in_forward_mode() || !has_tangent(grad), "the gradient carries a forward-mode tangent: there is no forward-mode derivative here");
   return grad.detach().resolve_neg();
 }
 
@@ -314,10 +317,11 @@ struct List {
     address.reserve(tensors.size());
     size.reserve(tensors.size());
     dtype.reserve(tensors.size());
+    const bool forward_mode = in_forward_mode();
     for (const auto& entry : tensors) {
       if (!entry.has_value()) continue;
       const Tensor& t = *entry;
-      REQUIRE(!has_tangent(t), "tensors carry a forward-mode tangent: there is no forward-mode derivative here");
+      REQUIRE(!forward_mode || !has_tangent(t), "tensors carry a forward-mode tangent: there is no forward-mode derivative here");
       REQUIRE(t.defined() && t.is_cuda(), "tensors must be CUDA tensors (this library has no CPU path)");
       REQUIRE(t.layout() == at::kStrided && dtype_of(t) >= 0,
               "tensors must be dense float16, bfloat16, float32 or float64 tensors");
@@ -372,12 +376,14 @@ Tensor clip_grad_norm(const std::vector<std::optional<Tensor>>& tensors, double 
   if (!list.first) return no_norm();
   std::vector<void*> to;
   to.reserve(list.address.size());
+  const bool forward_mode = in_forward_mode();
   for (size_t i = 0; i < tensors.size(); ++i) {
     if (!tensors[i].has_value()) continue;
     const Tensor& t = *tensors[i];
     if (out) {
       const auto& o = (*out)[i];
-      REQUIRE(!o.has_value() || !has_tangent(*o), "out carries a forward-mode tangent: there is no forward-mode derivative here");
+      REQUIRE(!forward_mode || !o.has_value() || !has_tangent(*o),
+              "out carries a forward-mode tangent: there is no forward-mode derivative here");
       REQUIRE(o.has_value() && o->defined() && o->layout() == at::kStrided && !o->is_neg() && o->device() == t.device() &&
                   o->scalar_type() == t.scalar_type() && o->sizes() == t.sizes() && same_order(*o, t),
               "out must match tensors in device, type, shape and strides");
