@@ -348,15 +348,16 @@ TBE_API int tbe_expert_combine_backward(const void* grad_out, int64_t grad_strid
 /* ---- gradients: global norm and clipping ----------------------------------- */
 
 /* norm (device, one float; inf where it passes fp32's range) = sqrt(sum of squares over all elements of
- * `count` tensors), summed in fp64 in a fixed order.  tensors, numels and dtypes are HOST arrays, read during the call; every tensor is dense
+ * `count` tensors), summed in fp64 in a fixed order (16-bit values eight at a time in fp32).  tensors, numels and dtypes are HOST arrays, read during the call; every tensor is dense
  * memory of numels[i] elements (0 is allowed) on the current device.  The table travels in the kernels'
  * parameters, 1024 tensors per launch. */
 TBE_API int64_t tbe_grad_norm_workspace_bytes(int64_t count);
 TBE_API int tbe_grad_norm(const void* const* tensors, const int64_t* numels, const int32_t* dtypes, int64_t count,
                           float* norm, void* workspace, int64_t workspace_bytes, void* stream);
-/* outputs[i] = min(1, max_norm / (norm + eps)) * tensors[i], rounded once; outputs[i] == tensors[i] is in
- * place.  A norm of NaN makes everything NaN, an infinite one zeroes the finite elements, as the formula
- * says.  With every tensor in place and a factor of 1 nothing is stored.  An output that shares memory
+/* outputs[i] = min(1, max_norm / (norm + eps)) * tensors[i]: the factor in fp64, rounded to fp32, the product
+ * in fp32 and its rounding to the element's type (all in fp64 for TBE_F64); outputs[i] == tensors[i] is in
+ * place.  A norm of NaN makes everything NaN, one that is infinite in fp64 zeroes the finite elements, as the
+ * formula says.  With every tensor in place and a factor of 1 nothing is stored.  An output that shares memory
  * with another tensor of the list is refused. */
 TBE_API int tbe_grad_clip(const void* const* tensors, void* const* outputs, const int64_t* numels, const int32_t* dtypes,
                           int64_t count, double max_norm, double eps, float* norm, void* workspace,

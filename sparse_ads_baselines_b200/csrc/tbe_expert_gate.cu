@@ -16,12 +16,15 @@
 // first, by k rounds over the lanes' maxima alone; their values are dealt to all lanes, C = k V / 32 each
 // (2 or 4), and k rounds over those give the choices.  Groups of fewer lanes, and a k V above 128, run the
 // rounds over all keys: sorted in runs of eight (a 19-comparator network), a round compares the runs' heads
-// and pops one.  Nothing but the logits is read and nothing is kept for the backward, which recomputes the
-// row's maximum and sum from the logits when it needs them.
+// and pops one.  The backward takes the gate's own weights and ids; only the whole-row softmax reads the logits
+// again and recomputes the row's maximum and sum.
 //
 // Bound by instruction issue (78 % of the slots), not by HBM.  65536 rows of 256 bf16 logits, k = 8, are
 // 33.5 MB (5 us) and take 25 us: 33 us with rounds over the sorted runs of all keys, 30 with the best lanes
-// first, 25 with four rows per warp.  fp32: 45 us.  One row: 2.4 us, about an empty kernel's time.
+// first, 25 with four rows per warp (29 with the whole row's softmax).  fp32: 45 us (48).  Rows that are no multiple
+// of 16 bytes take one element per load: 60 bf16 experts, k = 4, 11.3 us against 9.2 for 64, 100 21.4 against 17.2
+// for 96 or 104.  One row: 2.4 us, about an empty kernel's time.  The fp64 variants with 128-bit keys spill (64 to
+// 92 bytes) in a warp per row.
 #include "tbe_elem.cuh"
 
 namespace tbe {

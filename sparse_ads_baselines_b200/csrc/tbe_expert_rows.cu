@@ -238,7 +238,8 @@ struct Vectors {
 // A thread takes U vectors of one sample's row, so that a warp's loads stay contiguous and the positions are
 // looked up once for all of them: U independent loads, then k stores each.
 // 2048 rows of 8192 fp16, k = 2: 16 us for 101 MB (6.3 TB/s).  Rows that are only aligned to 4 bytes are
-// bound by the load-store unit: 5003 of 1001 fp32, k = 6: 26 us for 140 MB (5.4 TB/s; 29 without TILED).
+// bound by the load-store unit: 5003 of 1001 fp32, k = 6: 26 us for 140 MB (5.4 TB/s; 29 without TILED); to 2 bytes:
+// 8192 of 2047 bf16, k = 4: 40 us, 27 for 2048.
 template <int VB, int U, bool TILED>
 __global__ void __launch_bounds__(256) dispatch_kernel(RowArgs a) {
   const uint32_t i = blockIdx.x * 256u + threadIdx.x;
@@ -263,7 +264,9 @@ __global__ void __launch_bounds__(256) dispatch_kernel(RowArgs a) {
 }
 
 // The same U vectors, summed over the sample's rows; KB * U row loads are in flight together, in 64 registers
-// (four CTAs per SM).  8192 rows of 2048 bf16, us for (KB, U) = (1, 4) / (2, 1) / (2, 2) / (4, 1) / (4, 2) / (8, 1):
+// (four CTAs per SM), which do not hold all of them in 16-bit types with 16-byte vectors: (U, KB) = (2, 4) spills 96
+// bytes where it is not TILED (k > 2, rows of fewer than 64 vectors: 65536 of 256 bf16, k = 8, 55 us for a floor of
+// 46), (4, 1) 8 or 40.  8192 rows of 2048 bf16, us for (KB, U) = (1, 4) / (2, 1) / (2, 2) / (4, 1) / (4, 2) / (8, 1):
 // k = 1 10.8 / 16.5 / 12.7 / 19.5 / 13.8 / 23.8, k = 2 15.9 / 18.9 / 15.5 / 22.4 / 16.6 / 25.7, k = 4 25.7 / 28.8 /
 // 24.5 / 26.6 / 23.4 / 30.2, k = 8 45.9 / 49.0 / 43.3 / 44.4 / 41.7 / 42.6 (302 MB: 7.2 TB/s with L2's help).
 template <typename T, int VB, int U, int KB, bool TILED>

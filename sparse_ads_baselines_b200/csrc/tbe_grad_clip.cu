@@ -209,7 +209,7 @@ __device__ void scale_chunk(const T* src, T* dst, int n, double c, int me, int t
   constexpr int NV = 16 / sizeof(T);
   const Split<A> f = split<A>(c);
   const uintptr_t s = reinterpret_cast<uintptr_t>(src), d = reinterpret_cast<uintptr_t>(dst);
-  if ((s ^ d) & 15) {  // no vector of one is a vector of the other
+  if ((s ^ d) & 15) {  // no vector of one is a vector of the other (50 M bf16 elements: 185 us, 32 for aligned ones)
     for (int i = me; i < n; i += threads) dst[i] = from_acc<T>(to_acc<T>(src[i]) * f.a * f.b);
     return;
   }
@@ -284,6 +284,7 @@ struct Owners {
 // through distributed shared memory between the two passes.  The second launch of the two-kernel form costs
 // the host 4 us and the GPU a gap of about 1.5; on the GPU itself (one kernel / the two without the gap) 40 fp32
 // tensors of 1000 elements in all take 5.0 / 5.7 us, of 65536 7.5 / 5.8, of 131072 7.2 / 5.7, of 262144 11.0 / 6.7.
+// (1024 threads leave 64 registers; 32 bytes spill.)
 template <int CAP>
 __global__ void __launch_bounds__(1024) grad_clip_small_kernel(const __grid_constant__ Table<CAP> t,
                                                                const __grid_constant__ Owners<CAP> owners, bool scale,

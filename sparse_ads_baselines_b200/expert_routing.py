@@ -11,7 +11,8 @@ the router, and ``plan`` the sort that its backward makes.  All four are differe
 sense (``gate`` in its logits, ``dispatch`` in ``x``, ``combine`` in ``y`` and ``weights``), once; nothing
 synchronises, no size depends on the data, and no result depends on the order in which a GPU serves
 atomics.  float16, bfloat16, float32 and float64; weights are float32 (float64 for float64).  Everything is
-enqueued on the current CUDA stream of the tensors' device.  There is no CPU path.
+enqueued on the current CUDA stream of the tensors' device.  There is no CPU path.  Forward-mode tangents are
+refused, and so is recording by torch.jit.trace or make_fx; torch.compile leaves the graph around a call.
 
 A choice of ``-1`` (or any id outside ``0 .. num_experts-1``, for instance an expert of another rank) is
 nobody's: its row lies behind ``p.offsets[-1]``, ``dispatch`` fills it with zeros and ``combine`` leaves it
