@@ -8,6 +8,7 @@
 #include <pybind11/stl.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -15,6 +16,7 @@
 #include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/jit/frontend/tracer.h>
+#include <torch/csrc/jit/ir/ir.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
@@ -64,11 +66,20 @@ int dtype_of(const Tensor& t) {
 at::ScalarType weights_type(const Tensor& rows) { return rows.scalar_type() == at::kDouble ? at::kDouble : at::kFloat; }
 
 // A recorder sees the allocation of an output but not the kernel that fills it: what it records returns memory that
-// nobody wrote.
+// nobody wrote.  Inside a Python autograd.Function (or a custom operator), which torch.jit.trace records as a whole and
+// calls again, there is nothing to refuse.
+bool jit_records_this() {
+  if (!torch::jit::tracer::isTracing() || !at::tracer::impl::is_dispatch_enabled()) return false;
+  // a Function gets its outputs when its forward has returned
+  for (const torch::jit::Node* n : torch::jit::tracer::getTracingState()->graph->nodes())
+    if (n->kind() == torch::jit::prim::PythonOp && n->outputs().empty()) return false;
+  return true;
+}
 void refuse_recording() {
-  using Modes = c10::impl::TorchDispatchModeTLS;
-  REQUIRE(!torch::jit::tracer::isTracing() && !Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
-          "expert routing and gradient clipping cannot be recorded (torch.jit.trace, make_fx, torch.export)");
+  REQUIRE(!jit_records_this() &&
+              !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+          "expert routing and gradient clipping cannot be recorded (torch.jit.trace, make_fx, torch.export): wrap the "
+          "call in an operator that the recorder keeps as a whole");
 }
 
 // Forward-mode differentiation keeps a tangent beside the tensor; what the kernels compute would come without one,

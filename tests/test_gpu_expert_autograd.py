@@ -126,3 +126,30 @@ def test_renormalized_gradient_without_logits(cuda_device, dtype):
         _lib.call("tbe_expert_gate_backward", g.data_ptr(), logits, stride, w.data_ptr(), e.data_ptr(), out.data_ptr(),
                   33, 48, 4, kind, 1, stream)
         assert torch.equal(out, want)
+
+
+class _Weights(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x):
+        return er.gate(x, 2)[0]
+
+
+@torch.library.custom_op("routing_tests::gate_weights", mutates_args=())
+def _gate_weights(x: torch.Tensor) -> torch.Tensor:
+    return er.gate(x, 2)[0]
+
+
+@_gate_weights.register_fake
+def _(x):
+    return x.new_empty(x.shape[0], 2, dtype=torch.float32)
+
+
+def test_operators_that_a_recorder_keeps_as_a_whole(cuda_device):
+    """A call inside a Python autograd.Function or a custom operator is part of what is recorded, and runs again."""
+    x, other = torch.randn(2, 5, 6, device=cuda_device)
+    want = er.gate(other, 2)[0] * 2
+    for f in (torch.jit.trace(lambda t: _Weights.apply(t) * 2, x, check_trace=False),
+              torch.jit.trace(lambda t: _gate_weights(t) * 2, x, check_trace=False),
+              make_fx(lambda t: _gate_weights(t) * 2)(x),
+              torch.compile(lambda t: _gate_weights(t) * 2, backend="eager", fullgraph=True)):
+        assert torch.equal(f(other), want)

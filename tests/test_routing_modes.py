@@ -54,3 +54,37 @@ def test_recording_is_refused(op, recorder):
         RECORDERS[recorder](RECORDED[op], torch.zeros(4, 6))
     with pytest.raises(RuntimeError, match="CUDA tensor"):  # and not refused once the recorder is gone
         RECORDED[op](torch.zeros(4, 6))
+
+
+class _Wrapped(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x):
+        return er.gate(x, 2)[0]
+
+
+def test_a_recorded_function_is_not_refused():
+    """torch.jit.trace keeps a Python autograd.Function as a whole and calls it again, so its result is computed."""
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        torch.jit.trace(_Wrapped.apply, torch.zeros(4, 6), check_trace=False)
+
+
+class _WithTangent(torch.autograd.Function):
+    @staticmethod
+    def forward(x):
+        return er.gate(x, 2)[0]
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        pass
+
+    @staticmethod
+    def jvp(ctx, t):
+        return t[:, :2]
+
+
+def test_a_function_with_its_own_forward_mode_is_not_refused():
+    """Inside its forward the tangents are its own business."""
+    with fwd.dual_level():
+        x = fwd.make_dual(torch.zeros(4, 6), torch.ones(4, 6))
+        with pytest.raises(RuntimeError, match="CUDA tensor"):
+            _WithTangent.apply(x)
