@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(kGateThreads) gate_backward_chosen_kernel(Gate
 // which keeps its digits when one weight is nearly 1 and c nearly that slot's g.  The lanes that hold the slots mark
 // their columns in the owners' masks; the owners store -p_j c everywhere in wide stores and then, behind a barrier of
 // the warp, the slots' lanes w_s times the sum above on the chosen columns.  Bound by instruction issue: 65536 rows of
-// 256, k = 8: 33.2 us in bf16, 33.7 in fp32 (8192 rows of 1000 fp32: 14.7); with a division per column, the columns' factors
+// 256, k = 8: 33.2 us in bf16, 35.0 in fp32 (8192 rows of 1000 fp32: 14.9); with a division per column, the columns' factors
 // read back from shared memory and the logits loaded behind the slots 41.6, 44.3 and 25.5, and 31.6, 35.1 and 19.5
 // before the rest's mass was summed at all.
 template <typename T, int V, int VE>
@@ -504,9 +504,10 @@ __global__ void __launch_bounds__(kGateThreads) gate_backward_kernel(GateArgs a)
     rest += ((picked >> i) & 1u) ? A(0) : p[i];
   }
   sum = group_sum(sum, glog);
-  const A scale = none && !isnan(sum) ? A(0) : A(1) / sum;  // one division per row: p_j = p[i] * scale
-  rest = group_sum(rest, glog) * scale;
-  const A spread = scale * (A(0) - c);
+  rest = group_sum(rest, glog);
+  const bool nothing = none && !isnan(sum);  // every logit is -inf: p[i] is 0
+  rest = nothing ? A(0) : rest / sum;
+  const A spread = nothing ? A(0) : (A(0) - c) / sum;  // two divisions a row instead of one a column
 #pragma unroll
   for (int i = 0; i < V; i += VE) {
     const int col0 = column<VE>(i, sub, glog);
